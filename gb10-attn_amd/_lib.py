@@ -29,7 +29,9 @@ EXPORTS = (
     "paged_attention_prefill", "paged_attention_prefill_wmma", "paged_attention_prefill_wmma_scaled",
     "paged_attention_prefill_varlen", "paged_attention_prefill_varlen_scaled",
     "paged_attention_prefill_split", "paged_attention_prefill_workspace_size",
-    "pa_write_kv", "pa_write_kv_scaled",
+    "pa_write_kv", "pa_write_kv_scaled", "pa_qk_norm_rope_write_kv",
+    "pa_copy_pages", "pa_fork_sequences", "pa_fork_workspace_size", "pa_free_sequences",
+    "pa_compact_pages", "pa_compact_workspace_size",
 )
 
 
@@ -113,6 +115,20 @@ def lib() -> C.CDLL:
     L.pa_write_kv.argtypes = [T, T, T, T, T, P]
     L.pa_write_kv_scaled.restype = C.c_int
     L.pa_write_kv_scaled.argtypes = [T, T, T, T, T, C.c_double, C.c_double, P]
+    L.pa_qk_norm_rope_write_kv.restype = C.c_int
+    L.pa_qk_norm_rope_write_kv.argtypes = [T] * 11 + [C.c_double, C.c_int, C.c_double, C.c_double, P]
+    L.pa_copy_pages.restype = C.c_int
+    L.pa_copy_pages.argtypes = [T] * 4 + [P]
+    L.pa_fork_sequences.restype = C.c_int
+    L.pa_fork_sequences.argtypes = [T] * 8 + [P, sz, P]
+    L.pa_fork_workspace_size.restype = sz
+    L.pa_fork_workspace_size.argtypes = [T, T, T]
+    L.pa_free_sequences.restype = C.c_int
+    L.pa_free_sequences.argtypes = [T] * 4 + [i64, P]
+    L.pa_compact_pages.restype = C.c_int
+    L.pa_compact_pages.argtypes = [T] * 8 + [P, sz, P]
+    L.pa_compact_workspace_size.restype = sz
+    L.pa_compact_workspace_size.argtypes = [T]
     _lib = L
     return L
 

@@ -1232,3 +1232,336 @@ int pa_write_kv_scaled(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tens
 }
 
 }  // extern "C"
+
+// ------------------------------------------------- norm, rotation and write --
+
+static bool act_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
+
+// A [rows, heads, D] (n = 2) or [NB, BS, HKV, D] (n = 3) view the row kernels
+// address: last dimension contiguous, base and outer strides 16-byte aligned.
+static int check_rows(const pa_tensor_t* t, const char* name, int n) {
+  const int es = dtype_bytes(t->dtype);
+  if (t->stride[n] != 1) return fail(PA_ERR_INVALID_ARGUMENT, "%s must have a contiguous last dimension", name);
+  for (int i = 0; i < n; ++i) {
+    if (t->stride[i] < 0) return fail(PA_ERR_UNSUPPORTED, "%s strides must be non-negative", name);
+    if (((t->stride[i] * es) & 15) != 0 && t->shape[i] > 1)
+      return fail(PA_ERR_UNSUPPORTED, "%s strides must be multiples of 16 bytes", name);
+  }
+  if (!aligned16(t->data)) return fail(PA_ERR_UNSUPPORTED, "%s must be 16-byte aligned", name);
+  return PA_OK;
+}
+
+static int check_index(const pa_tensor_t* t, const char* name, int64_t n, bool i64_too) {
+  int rc = check_tensor(t, name, 1, "a vector");
+  if (rc) return rc;
+  if (t->dtype != kI32 && !(i64_too && t->dtype == kI64))
+    return fail(PA_ERR_INVALID_ARGUMENT, i64_too ? "%s must be int32 or int64" : "%s must be int32", name);
+  if (n >= 0 && t->shape[0] != n) return fail(PA_ERR_INVALID_ARGUMENT, "%s must have %lld entries", name, (long long)n);
+  if (t->shape[0] > 1 && t->stride[0] != 1) return fail(PA_ERR_INVALID_ARGUMENT, "%s must be contiguous", name);
+  return PA_OK;
+}
+
+extern "C" int pa_qk_norm_rope_write_kv(pa_tensor_t* q_out, pa_tensor_t* k_cache, pa_tensor_t* v_cache,
+                                        const pa_tensor_t* q, const pa_tensor_t* key, const pa_tensor_t* value,
+                                        const pa_tensor_t* slot_mapping, const pa_tensor_t* cos_sin,
+                                        const pa_tensor_t* positions, const pa_tensor_t* q_weight,
+                                        const pa_tensor_t* k_weight, double eps, int interleaved, double k_scale,
+                                        double v_scale, void* stream) {
+  g_launches.clear();
+  int rc;
+  if ((rc = check_tensor(q, "q", 3, "[T, H, D]"))) return rc;
+  if ((rc = check_tensor(q_out, "q_out", 3, "[T, H, D]"))) return rc;
+  if ((rc = check_tensor(key, "key", 3, "[T, HKV, D]"))) return rc;
+  if ((rc = check_tensor(value, "value", 3, "[T, HKV, D]"))) return rc;
+  if ((rc = check_tensor(k_cache, "k_cache", 4, "[NB, BS, HKV, D]"))) return rc;
+  if ((rc = check_tensor(v_cache, "v_cache", 4, "[NB, BS, HKV, D]"))) return rc;
+  if ((rc = check_tensor(cos_sin, "cos_sin", 2, "[positions, rot]"))) return rc;
+  const int64_t T = q->shape[0], H = q->shape[1], D = q->shape[2];
+  const int64_t NB = k_cache->shape[0], BS = k_cache->shape[1], HKV = k_cache->shape[2];
+  if (!act_dtype(q->dtype))
+    return fail(PA_ERR_INVALID_ARGUMENT, "q must be float32, float16 or bfloat16 (got %s)", dtype_name(q->dtype));
+  if (key->dtype != q->dtype || value->dtype != q->dtype)
+    return fail(PA_ERR_INVALID_ARGUMENT, "key and value must have the dtype of q");
+  if (!act_dtype(q_out->dtype))
+    return fail(PA_ERR_INVALID_ARGUMENT, "q_out must be float32, float16 or bfloat16 (got %s)", dtype_name(q_out->dtype));
+  const int cd = k_cache->dtype;
+  if (!act_dtype(cd) && cd != kFP8)
+    return fail(PA_ERR_INVALID_ARGUMENT, "k_cache must be float16, bfloat16, float32 or float8_e4m3fn (got %s)",
+                dtype_name(cd));
+  if (v_cache->dtype != cd) return fail(PA_ERR_INVALID_ARGUMENT, "v_cache must have the dtype of k_cache");
+  for (int i = 0; i < 3; ++i)
+    if (q_out->shape[i] != q->shape[i]) return fail(PA_ERR_INVALID_ARGUMENT, "q_out must have the shape of q");
+  for (int i = 0; i < 4; ++i)
+    if (v_cache->shape[i] != k_cache->shape[i])
+      return fail(PA_ERR_INVALID_ARGUMENT, "v_cache must have the shape of k_cache");
+  for (const pa_tensor_t* t : {key, value})
+    if (t->shape[0] != T || t->shape[1] != HKV || t->shape[2] != D)
+      return fail(PA_ERR_INVALID_ARGUMENT, "key and value must be [%lld, %lld, %lld]", (long long)T, (long long)HKV,
+                  (long long)D);
+  if (k_cache->shape[3] != D)
+    return fail(PA_ERR_INVALID_ARGUMENT, "k_cache head_dim (%lld) != q head_dim (%lld)", (long long)k_cache->shape[3],
+                (long long)D);
+  if (D <= 0 || D % 16 != 0 || D > 256)
+    return fail(PA_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 up to 256 (got %lld)", (long long)D);
+  const int64_t rot = cos_sin->shape[1];
+  if (rot > D) return fail(PA_ERR_INVALID_ARGUMENT, "cos_sin has more columns than head_dim");
+  if (rot % 16 != 0) return fail(PA_ERR_UNSUPPORTED, "cos_sin must have a multiple of 16 columns");
+  if (!act_dtype(cos_sin->dtype))
+    return fail(PA_ERR_INVALID_ARGUMENT, "cos_sin must be float32, float16 or bfloat16");
+  if ((rc = check_index(slot_mapping, "slot_mapping", T, true))) return rc;
+  if ((rc = check_index(positions, "positions", T, true))) return rc;
+  int wd = -1;
+  for (const pa_tensor_t* w : {q_weight, k_weight}) {
+    if (!w) continue;
+    if ((rc = check_tensor(w, "q_weight/k_weight", 1, "[D]"))) return rc;
+    if (w->shape[0] != D) return fail(PA_ERR_INVALID_ARGUMENT, "q_weight/k_weight must have head_dim entries");
+    if (!act_dtype(w->dtype) || (wd >= 0 && w->dtype != wd))
+      return fail(PA_ERR_INVALID_ARGUMENT, "q_weight and k_weight must share a type: float32, float16 or bfloat16");
+    wd = w->dtype;
+    if ((rc = check_rows(w, "q_weight/k_weight", 0))) return rc;
+  }
+  if (!finite_f32(eps) || eps < 0) return fail(PA_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (!finite_f32(k_scale) || !finite_f32(v_scale) || (float)k_scale == 0.0f || (float)v_scale == 0.0f)
+    return fail(PA_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be finite and nonzero");
+  if (BS <= 0) return fail(PA_ERR_INVALID_ARGUMENT, "block_size must be positive");
+  if (NB * BS >= (1LL << 31) || T > INT32_MAX || H >= (1 << 20) || HKV >= (1 << 20))
+    return fail(PA_ERR_UNSUPPORTED, "problem too large for 32-bit slot indices");
+  if ((rc = check_rows(q, "q", 2)) || (rc = check_rows(q_out, "q_out", 2)) || (rc = check_rows(key, "key", 2)) ||
+      (rc = check_rows(value, "value", 2)) || (rc = check_rows(k_cache, "k_cache", 3)) ||
+      (rc = check_rows(v_cache, "v_cache", 3)) || (rot > 0 && (rc = check_rows(cos_sin, "cos_sin", 1))))
+    return rc;
+  if (T == 0 || H + HKV == 0) return PA_OK;
+  RopeParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = q->data; p.key = key->data; p.value = value->data; p.q_out = q_out->data;
+  p.kc = k_cache->data; p.vc = v_cache->data;
+  p.q_weight = q_weight ? q_weight->data : nullptr;
+  p.k_weight = k_weight ? k_weight->data : nullptr;
+  p.table = cos_sin->data; p.positions = positions->data; p.slots = slot_mapping->data;
+  p.q_st = q->stride[0]; p.q_sh = q->stride[1];
+  p.key_st = key->stride[0]; p.key_sh = key->stride[1];
+  p.val_st = value->stride[0]; p.val_sh = value->stride[1];
+  p.out_st = q_out->stride[0]; p.out_sh = q_out->stride[1];
+  p.kc_sb = k_cache->stride[0]; p.kc_st = k_cache->stride[1]; p.kc_sh = k_cache->stride[2];
+  p.vc_sb = v_cache->stride[0]; p.vc_st = v_cache->stride[1]; p.vc_sh = v_cache->stride[2];
+  p.table_st = cos_sin->stride[0]; p.table_rows = cos_sin->shape[0];
+  p.nslots = NB * BS;
+  p.T = (int32_t)T; p.H = (int32_t)H; p.HKV = (int32_t)HKV; p.D = (int32_t)D; p.BS = (int32_t)BS;
+  p.rot = (int32_t)rot; p.interleaved = interleaved != 0;
+  p.act_dtype = q->dtype; p.cache_dtype = cd; p.out_dtype = q_out->dtype;
+  p.weight_dtype = wd; p.table_dtype = cos_sin->dtype;
+  p.slot_i64 = slot_mapping->dtype == kI64; p.pos_i64 = positions->dtype == kI64;
+  p.k_scale = (float)k_scale; p.v_scale = (float)v_scale;
+  p.k_rcp = 1.0f / p.k_scale; p.v_rcp = 1.0f / p.v_scale;
+  auto in_range = [](float r) { return std::fabs(r) >= 0x1p-60f && std::fabs(r) <= 0x1p60f; };
+  p.k_fast = in_range(p.k_rcp); p.v_fast = in_range(p.v_rcp);
+  p.unit_scale = p.k_scale == 1.0f && p.v_scale == 1.0f;
+  p.eps = (float)eps; p.inv_d = 1.0f / (float)D;
+  p.bs_div = make_fastdiv((uint32_t)BS);
+  return hip_status(launch_qk_norm_rope(p, static_cast<hipStream_t>(stream)), "norm and rotation kernel launch");
+}
+
+// ------------------------------------------------------------------- pages --
+
+static int check_pool(const pa_tensor_t* k, const pa_tensor_t* v, PagePool* c) {
+  int rc;
+  if ((rc = check_tensor(k, "k_cache", 4, "[L, NB, BS, row]"))) return rc;
+  if (v && (rc = check_tensor(v, "v_cache", 4, "[L, NB, BS, row]"))) return rc;
+  const int es = dtype_bytes(k->dtype);
+  if (es == 0) return fail(PA_ERR_INVALID_ARGUMENT, "k_cache has an unknown type");
+  if (v && v->dtype != k->dtype) return fail(PA_ERR_INVALID_ARGUMENT, "v_cache must have the dtype of k_cache");
+  for (int i = 0; v && i < 4; ++i)
+    if (v->shape[i] != k->shape[i]) return fail(PA_ERR_INVALID_ARGUMENT, "v_cache must have the shape of k_cache");
+  const int64_t L = k->shape[0], NB = k->shape[1], BS = k->shape[2], W = k->shape[3];
+  if (BS <= 0) return fail(PA_ERR_INVALID_ARGUMENT, "block_size must be positive");
+  if ((W * es) % 16 != 0) return fail(PA_ERR_UNSUPPORTED, "a token's row must be a multiple of 16 bytes");
+  if (NB >= (1LL << 31) - 4096 || L >= (1 << 20) || W * es / 16 >= (1LL << 31) || BS >= (1LL << 31) ||
+      BS * (W * es / 16) >= (1LL << 31) - kMaxPiece)
+    return fail(PA_ERR_UNSUPPORTED, "cache too large for 32-bit page indices");
+  for (const pa_tensor_t* t : {k, v}) {
+    if (!t) continue;
+    if ((rc = check_rows(t, t == k ? "k_cache" : "v_cache", 3))) return rc;
+    for (int i = 0; i < 3; ++i)
+      if (t->shape[i] > 1 && t->stride[i] == 0)
+        return fail(PA_ERR_INVALID_ARGUMENT, "k_cache/v_cache pages must not overlap");
+  }
+  memset(c, 0, sizeof(*c));
+  c->k = static_cast<char*>(k->data);
+  c->k_sl = k->stride[0] * es; c->k_sb = k->stride[1] * es; c->k_st = k->stride[2] * es;
+  if (v) {
+    c->v = static_cast<char*>(v->data);
+    c->v_sl = v->stride[0] * es; c->v_sb = v->stride[1] * es; c->v_st = v->stride[2] * es;
+  }
+  c->num_blocks = NB;
+  c->L = (int32_t)L; c->BS = (int32_t)BS; c->row16 = (int32_t)(W * es / 16);
+  c->planes = (int32_t)(v ? 2 * L : L);
+  c->row_div = make_fastdiv((uint32_t)std::max(1, c->row16));
+  return PA_OK;
+}
+
+static int check_tables(const pa_tensor_t* t, const char* name) {
+  int rc = check_tensor(t, name, 2, "[R, MB]");
+  if (rc) return rc;
+  if (t->dtype != kI32) return fail(PA_ERR_INVALID_ARGUMENT, "%s must be int32", name);
+  if ((t->shape[1] > 1 && t->stride[1] != 1) || (t->shape[0] > 1 && t->stride[0] < t->shape[1]))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s rows must be contiguous", name);
+  if (t->shape[0] >= (1LL << 31) || t->shape[1] >= (1LL << 31))
+    return fail(PA_ERR_UNSUPPORTED, "%s is too large", name);
+  return PA_OK;
+}
+
+static int check_scratch(size_t need, const void* ws, size_t bytes) {
+  if (need > 0 && (!ws || bytes < need))
+    return fail(PA_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, ws ? bytes : 0);
+  if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
+    return fail(PA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  return PA_OK;
+}
+
+static size_t fork_bytes(int64_t N, int64_t MB, int64_t NB) { return 4 * ((size_t)N * MB + 3 * (size_t)N + NB); }
+static int64_t compact_blocks(int64_t NB) { return (NB + kCompactPages - 1) / kCompactPages; }
+static size_t compact_bytes(int64_t NB) { return 4 * ((size_t)compact_blocks(NB) + 2 * (size_t)NB + 1); }
+
+// Tables, lengths, counts and rows of a fork or a release.
+static int fork_args(ForkParams* p, const pa_tensor_t* bt, const pa_tensor_t* lens, const pa_tensor_t* refs,
+                     const pa_tensor_t* rows, int64_t BS) {
+  int rc;
+  if ((rc = check_tables(bt, "block_tables"))) return rc;
+  const int64_t R = bt->shape[0], MB = bt->shape[1];
+  if ((rc = check_index(lens, "context_lens", R, false)) || (rc = check_index(refs, "page_refs", -1, false)) ||
+      (rc = check_index(rows, "rows", -1, false)))
+    return rc;
+  if (BS <= 0) return fail(PA_ERR_INVALID_ARGUMENT, "block_size must be positive");
+  if (BS >= (1LL << 31) || MB * BS >= (1LL << 31)) return fail(PA_ERR_UNSUPPORTED, "problem too large for 32-bit token indices");
+  if (rows->shape[0] > kForkMax) return fail(PA_ERR_UNSUPPORTED, "at most %lld rows per call", (long long)kForkMax);
+  p->tables = static_cast<int32_t*>(bt->data);
+  p->lens = static_cast<int32_t*>(lens->data);
+  p->refs = static_cast<int32_t*>(refs->data);
+  p->rows = static_cast<const int32_t*>(rows->data);
+  p->tb_stride = R > 1 ? bt->stride[0] : MB;
+  p->N = (int32_t)rows->shape[0]; p->R = (int32_t)R; p->MB = (int32_t)MB; p->BS = (int32_t)BS;
+  p->bs_div = make_fastdiv((uint32_t)BS);
+  return PA_OK;
+}
+
+extern "C" int pa_copy_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* src,
+                             const pa_tensor_t* dst, void* stream) {
+  g_launches.clear();
+  CopyParams p;
+  int rc;
+  if ((rc = check_pool(k_cache, v_cache, &p.pool)) || (rc = check_index(src, "src", -1, false)) ||
+      (rc = check_index(dst, "dst", src->shape[0], false)))
+    return rc;
+  if (src->shape[0] >= (1LL << 24)) return fail(PA_ERR_UNSUPPORTED, "too many pages for one call");
+  p.src = static_cast<const int32_t*>(src->data);
+  p.dst = static_cast<const int32_t*>(dst->data);
+  p.N = (int32_t)src->shape[0];
+  if (p.N == 0 || p.pool.planes == 0 || p.pool.num_blocks == 0 || p.pool.row16 == 0) return PA_OK;
+  return hip_status(launch_copy_pages(p, static_cast<hipStream_t>(stream)), "page copy kernel launch");
+}
+
+extern "C" size_t pa_fork_workspace_size(const pa_tensor_t* block_tables, const pa_tensor_t* page_refs,
+                                         const pa_tensor_t* rows) {
+  if (check_tables(block_tables, "block_tables") || check_index(page_refs, "page_refs", -1, false) ||
+      check_index(rows, "rows", -1, false))
+    return (size_t)-1;
+  return fork_bytes(rows->shape[0], block_tables->shape[1], page_refs->shape[0]);
+}
+
+extern "C" int pa_fork_sequences(pa_tensor_t* k_cache, pa_tensor_t* v_cache, pa_tensor_t* block_tables,
+                                 pa_tensor_t* context_lens, pa_tensor_t* page_refs, const pa_tensor_t* parents,
+                                 const pa_tensor_t* rows, pa_tensor_t* copied, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  g_launches.clear();
+  ForkParams p;
+  memset(&p, 0, sizeof(p));
+  int rc;
+  if ((rc = check_pool(k_cache, v_cache, &p.pool)) ||
+      (rc = fork_args(&p, block_tables, context_lens, page_refs, rows, p.pool.BS)) ||
+      (parents && (rc = check_index(parents, "parents", p.N, false))) || (rc = check_index(copied, "copied", p.N, false)))
+    return rc;
+  if (page_refs->shape[0] != p.pool.num_blocks)
+    return fail(PA_ERR_INVALID_ARGUMENT, "page_refs must have one entry per page");
+  const size_t need = fork_bytes(p.N, p.MB, p.pool.num_blocks);
+  if (p.N == 0) return PA_OK;
+  if ((rc = check_scratch(need, workspace, workspace_bytes))) return rc;
+  p.parents = parents ? static_cast<const int32_t*>(parents->data) : nullptr;
+  p.result = static_cast<int32_t*>(copied->data);
+  p.ws_pages = static_cast<int32_t*>(workspace);
+  p.ws_len = p.ws_pages + (int64_t)p.N * p.MB;
+  p.ws_last = p.ws_len + p.N;
+  p.ws_new = p.ws_last + p.N;
+  p.ws_owner = p.ws_new + p.N;
+  return hip_status(launch_fork(p, static_cast<hipStream_t>(stream)), "fork kernel launch");
+}
+
+extern "C" int pa_free_sequences(pa_tensor_t* block_tables, pa_tensor_t* context_lens, pa_tensor_t* page_refs,
+                                 const pa_tensor_t* rows, int64_t block_size, void* stream) {
+  g_launches.clear();
+  ForkParams p;
+  memset(&p, 0, sizeof(p));
+  int rc;
+  if ((rc = fork_args(&p, block_tables, context_lens, page_refs, rows, block_size))) return rc;
+  p.pool.num_blocks = page_refs->shape[0];
+  if (p.N == 0) return PA_OK;
+  return hip_status(launch_free(p, static_cast<hipStream_t>(stream)), "free kernel launch");
+}
+
+extern "C" size_t pa_compact_workspace_size(const pa_tensor_t* page_refs) {
+  if (check_index(page_refs, "page_refs", -1, false)) return (size_t)-1;
+  return compact_bytes(page_refs->shape[0]);
+}
+
+// Byte range of a tensor with non-negative strides.
+static bool overlap(const pa_tensor_t* a, const pa_tensor_t* b) {
+  auto range = [](const pa_tensor_t* t, uintptr_t* lo, uintptr_t* hi) {
+    int64_t last = 0;
+    for (int i = 0; i < t->ndim; ++i) last += (t->shape[i] - 1) * t->stride[i];
+    *lo = reinterpret_cast<uintptr_t>(t->data);
+    *hi = numel(t) > 0 ? *lo + (uintptr_t)(last + 1) * dtype_bytes(t->dtype) : *lo;
+  };
+  uintptr_t al, ah, bl, bh;
+  range(a, &al, &ah);
+  range(b, &bl, &bh);
+  return al < bh && bl < ah;
+}
+
+extern "C" int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* block_tables,
+                                const pa_tensor_t* page_refs, pa_tensor_t* tables_out, pa_tensor_t* refs_out,
+                                pa_tensor_t* page_map, pa_tensor_t* num_live, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  g_launches.clear();
+  CompactParams p;
+  memset(&p, 0, sizeof(p));
+  int rc;
+  if ((rc = check_pool(k_cache, v_cache, &p.pool)) || (rc = check_tables(block_tables, "block_tables")) ||
+      (rc = check_tables(tables_out, "tables_out")))
+    return rc;
+  const int64_t NB = p.pool.num_blocks;
+  if ((rc = check_index(page_refs, "page_refs", NB, false)) || (rc = check_index(refs_out, "refs_out", NB, false)) ||
+      (rc = check_index(page_map, "page_map", NB, false)) || (rc = check_index(num_live, "num_live", 1, false)))
+    return rc;
+  const int64_t R = block_tables->shape[0], MB = block_tables->shape[1];
+  if (tables_out->shape[0] != R || tables_out->shape[1] != MB)
+    return fail(PA_ERR_INVALID_ARGUMENT, "tables_out must have the shape of block_tables");
+  p.tb_stride = R > 1 ? block_tables->stride[0] : MB;
+  p.tbo_stride = R > 1 ? tables_out->stride[0] : MB;
+  if (overlap(block_tables, tables_out) && (block_tables->data != tables_out->data || p.tb_stride != p.tbo_stride))
+    return fail(PA_ERR_INVALID_ARGUMENT, "tables_out must be block_tables or not overlap it");
+  if (overlap(page_refs, refs_out) && page_refs->data != refs_out->data)
+    return fail(PA_ERR_INVALID_ARGUMENT, "refs_out must be page_refs or not overlap it");
+  if (NB == 0) return fail(PA_ERR_INVALID_ARGUMENT, "k_cache must hold at least one block");
+  if ((rc = check_scratch(compact_bytes(NB), workspace, workspace_bytes))) return rc;
+  p.tables = static_cast<const int32_t*>(block_tables->data);
+  p.tables_out = static_cast<int32_t*>(tables_out->data);
+  p.refs = static_cast<const int32_t*>(page_refs->data);
+  p.refs_out = static_cast<int32_t*>(refs_out->data);
+  p.page_map = static_cast<int32_t*>(page_map->data);
+  p.num_live = static_cast<int32_t*>(num_live->data);
+  p.R = (int32_t)R; p.MB = (int32_t)MB; p.blocks = (int32_t)compact_blocks(NB);
+  p.ws_from = static_cast<int32_t*>(workspace);
+  p.ws_to = p.ws_from + NB;
+  p.ws_count = p.ws_to + NB;
+  p.ws_moves = p.ws_count + p.blocks;
+  return hip_status(launch_compact(p, static_cast<hipStream_t>(stream)), "compaction kernel launch");
+}

@@ -213,6 +213,95 @@ struct WriteParams {
   int32_t t_base;              // first token of this launch (large writes take several)
 };
 
+// Norm and rotation of new query and key heads, with the paged-cache write of
+// the keys and values (element strides).
+struct RopeParams {
+  const void* q;      // [T, H, D]
+  const void* key;    // [T, HKV, D]
+  const void* value;  // [T, HKV, D]
+  void* q_out;        // [T, H, D]
+  void* kc;           // k_cache / v_cache [NB, BS, HKV, D]
+  void* vc;
+  const void* q_weight;   // [D] or null (no norm)
+  const void* k_weight;   // [D] or null
+  const void* table;      // [rows, rot]: cosines, then sines
+  const void* positions;  // [T] int32 or int64
+  const void* slots;      // [T] int32 or int64
+  int64_t q_st, q_sh, key_st, key_sh, val_st, val_sh, out_st, out_sh;
+  int64_t kc_sb, kc_st, kc_sh, vc_sb, vc_st, vc_sh;
+  int64_t table_st, table_rows;
+  int64_t nslots;  // NB * BS (< 2^31)
+  int64_t t_base;  // first token of this launch
+  int32_t T, H, HKV, D, BS, rot, interleaved;
+  int32_t act_dtype, cache_dtype, out_dtype, weight_dtype, table_dtype, slot_i64, pos_i64;
+  int32_t unit_scale, k_fast, v_fast;  // as WriteParams
+  float k_scale, v_scale, k_rcp, v_rcp;
+  float eps, inv_d;
+  FastDiv bs_div, slice_div;
+};
+
+// Pages of the cache moved, forked and compacted.  A cache is [L, NB, BS, row]
+// with rows of row16 16-byte pieces (byte strides); v null: one cache.
+struct PagePool {
+  char* k;
+  char* v;
+  int64_t k_sl, k_sb, k_st;
+  int64_t v_sl, v_sb, v_st;
+  int64_t num_blocks;
+  int32_t L, BS, row16, planes;  // planes: L, or 2 L with v
+  FastDiv row_div;               // row16
+};
+
+constexpr int64_t kMaxPiece = 1024;  // 16-byte pieces of a page that a work-group moves at a time
+constexpr int64_t kForkMax = 65536;  // most rows of a fork or a release
+
+struct CopyParams {
+  PagePool pool;
+  const int32_t* src;  // [N]
+  const int32_t* dst;
+  int32_t N;
+};
+
+// Entry kinds and results of a fork.
+constexpr int32_t kForkNone = -1;     // row emptied, or forked without a copy
+constexpr int32_t kForkNoPage = -2;   // no free page: row emptied
+constexpr int32_t kForkInvalid = -3;  // entry refused
+
+struct ForkParams {
+  PagePool pool;
+  int32_t* tables;  // [R, MB]
+  int32_t* lens;    // [R]
+  int32_t* refs;    // [NB]
+  const int32_t* parents;  // [N]; null: every row is emptied
+  const int32_t* rows;     // [N]
+  int32_t* result;         // [N]: page copied to, or one of the codes above
+  int32_t* ws_pages;  // [N][MB] the parents' pages as the call found them
+  int32_t* ws_len;    // [N] new context (0: row emptied, -1: entry refused)
+  int32_t* ws_last;   // [N] page begun by the parent, -1: none
+  int32_t* ws_new;    // [N] its copy, -1: none
+  int32_t* ws_owner;  // [NB] lowest entry that takes a page over
+  int64_t tb_stride;
+  int32_t N, R, MB, BS;
+  FastDiv bs_div;
+};
+
+struct CompactParams {
+  PagePool pool;
+  const int32_t* tables;  // [R, MB]
+  int32_t* tables_out;
+  const int32_t* refs;  // [NB]
+  int32_t* refs_out;
+  int32_t* page_map;  // [NB]
+  int32_t* num_live;  // [1]
+  int32_t* ws_count;  // [blocks] live pages per block of kCompactPages
+  int32_t* ws_from;   // [NB] moved pages, ascending
+  int32_t* ws_to;     // [NB] the free pages they go to, ascending
+  int32_t* ws_moves;  // [1]
+  int64_t tb_stride, tbo_stride;
+  int32_t R, MB, blocks;
+};
+constexpr int kCompactPages = 2048;  // pages per work-group of the counting passes
+
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = 64 * kDecodeWaves;
 constexpr int kBtChunk = 256;  // block-table entries a decode work-group stages in LDS at a time
@@ -234,6 +323,11 @@ hipError_t launch_prefill_part(const PrefillParams& p, int kv_dtype, hipStream_t
 hipError_t launch_prefill32_part(const PrefillParams& p, int kv_dtype, hipStream_t stream);
 hipError_t launch_prefill32(const PrefillParams& p, int kv_dtype, hipStream_t stream);
 hipError_t launch_write_kv(const WriteParams& p, hipStream_t stream);
+hipError_t launch_qk_norm_rope(const RopeParams& p, hipStream_t stream);
+hipError_t launch_copy_pages(const CopyParams& p, hipStream_t stream);
+hipError_t launch_fork(const ForkParams& p, hipStream_t stream);
+hipError_t launch_free(const ForkParams& p, hipStream_t stream);
+hipError_t launch_compact(const CompactParams& p, hipStream_t stream);
 
 // Head packing (heads contiguous in the pool; MHA, or GQA groups of four over
 // 16-bit caches): one decode work-group

@@ -1,0 +1,464 @@
+// pa_pages.hip -- copying, forking, freeing and compacting the pages of a paged
+// cache on gfx950.
+//
+// State: the cache [L, NB, BS, row] (K and V), block tables [R, MB], context
+// lengths [R] and a count per page of the sequences that hold it (0: free).
+// Everything stays on the device, so a beam step or a compaction is a few
+// launches on the caller's stream with no answer to wait for.
+//
+//  * The data moves as bytes, 16 a load: HBM-bound, each page read and written
+//    once.  A work item is kPiece pieces of one page on one plane (a layer's K
+//    or V); a thread has kDepth pieces in flight.
+//  * The bookkeeping is exact and independent of the order in which work-groups
+//    run: counts change by integer atomics whose sum is all that matters, and
+//    whatever is handed out goes by index (the lowest free page to the first
+//    entry that needs one), through prefix sums.
+#include "pa_device.hpp"
+
+#include <algorithm>
+
+namespace pa {
+
+constexpr int kPgThreads = 256;
+constexpr int kDepth = 4;
+constexpr int kPiece = kPgThreads * kDepth;  // 16-byte pieces per work item
+static_assert(kPiece <= kMaxPiece, "checked by the host against 32-bit piece indices");
+constexpr int kScan = 1024;                  // threads of the allocating work-group
+
+__device__ inline int32_t load_now(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Pieces [first, first + kPiece) of page src of a plane, to page dst.
+__device__ inline void copy_item(const PagePool& c, int plane, int64_t src, int64_t dst, int first) {
+  const bool second = plane >= c.L;
+  const int64_t sb = second ? c.v_sb : c.k_sb, st = second ? c.v_st : c.k_st;
+  char* base = second ? c.v + (plane - c.L) * c.v_sl : c.k + plane * c.k_sl;
+  const char* from = base + src * sb;
+  char* to = base + dst * sb;
+  const int pieces = c.BS * c.row16;
+  u32x4_t x[kDepth];
+  int64_t at[kDepth];
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) {
+    const int n = first + i * kPgThreads + (int)threadIdx.x;
+    at[i] = -1;
+    if (n < pieces) {
+      const uint32_t row = fastdiv((uint32_t)n, c.row_div);
+      at[i] = (int64_t)row * st + (int64_t)(n - (int)row * c.row16) * 16;
+      x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(from + at[i]));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i)
+    if (at[i] >= 0) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4_t*>(to + at[i]));
+}
+
+__host__ __device__ inline int page_items(const PagePool& c) { return (c.BS * c.row16 + kPiece - 1) / kPiece; }
+
+// ------------------------------------------------------------------- copy --
+
+constexpr int kMaxGrid = 1 << 20;  // work-groups of a launch; the rest is a loop
+
+// A work item is kPiece pieces of one pair's page on one plane.  A destination
+// named twice takes the last pair that names it, whichever order the
+// work-groups run in.
+__global__ __launch_bounds__(kPgThreads) void copy_pages_kernel(const CopyParams p) {
+  const uint32_t items = (uint32_t)page_items(p.pool);
+  const int64_t all = (int64_t)p.N * p.pool.planes * items;
+  for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
+    const int64_t y = x / items;
+    const int first = (int)(x - y * items) * kPiece;
+    const int i = (int)(y / p.pool.planes), plane = (int)(y - (int64_t)i * p.pool.planes);
+    const int32_t src = p.src[i], dst = p.dst[i];
+    if (src < 0 || dst < 0 || src >= p.pool.num_blocks || dst >= p.pool.num_blocks || src == dst) continue;
+    int again = 0;
+    for (int j = i + 1 + (int)threadIdx.x; j < p.N; j += kPgThreads)
+      again |= p.dst[j] == dst && p.src[j] >= 0 && p.src[j] < p.pool.num_blocks;
+    if (__syncthreads_or(again)) continue;
+    copy_item(p.pool, plane, src, dst, first);
+  }
+}
+
+hipError_t launch_copy_pages(const CopyParams& p, hipStream_t stream) {
+  const int64_t all = (int64_t)p.N * p.pool.planes * page_items(p.pool);
+  note_launch("pa::copy_pages_kernel");
+  hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)std::min<int64_t>(all, kMaxGrid)), dim3(kPgThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------- fork --
+
+// Whether entry i is the first that names its row.
+__device__ inline bool first_of_row(const int32_t* rows, int i, int32_t row) {
+  int again = 0;
+  for (int j = threadIdx.x; j < i; j += kPgThreads) again |= rows[j] == row;
+  return !__syncthreads_or(again);
+}
+
+// Pages a row holds: those of its context, or none where it exceeds the table.
+__device__ inline int pages_of(const ForkParams& p, int32_t len) {
+  return len > 0 && (int64_t)len <= (int64_t)p.MB * p.BS ? (int)fastdiv((uint32_t)(len - 1), p.bs_div) + 1 : 0;
+}
+
+// One work-group per entry: the row's old pages are let go, the parent's whole
+// pages are counted once more and its pages kept aside, since another entry may
+// replace the parent's own row.  No table changes yet.
+__global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams p) {
+  const int i = blockIdx.x;
+  const int32_t row = p.rows[i];
+  const int64_t NB = p.pool.num_blocks;
+  const bool inside = row >= 0 && row < p.R;
+  if (!first_of_row(p.rows, i, row) || !inside) {  // (every thread takes the test's barrier)
+    if (threadIdx.x == 0) {
+      p.ws_len[i] = -1;
+      p.ws_last[i] = -1;
+      p.result[i] = kForkInvalid;
+    }
+    return;
+  }
+  const int32_t* old = p.tables + row * p.tb_stride;
+  const int held = pages_of(p, p.lens[row]);
+  for (int j = threadIdx.x; j < held; j += kPgThreads) {
+    const int32_t pg = old[j];
+    if (pg >= 0 && pg < NB) atomicAdd(p.refs + pg, -1);
+  }
+  const int32_t par = p.parents ? p.parents[i] : -1;
+  int32_t len = 0, last = -1, res = kForkNone;
+  if (par >= p.R) {
+    res = kForkInvalid;
+  } else if (par >= 0) {
+    len = max(p.lens[par], 0);
+    const int n = pages_of(p, len);
+    const int32_t* src = p.tables + par * p.tb_stride;
+    int bad = len > 0 && n == 0;
+    for (int j = threadIdx.x; j < n; j += kPgThreads) bad |= src[j] < 0 || src[j] >= NB;
+    bad = __syncthreads_or(bad);
+    if (bad) {
+      len = 0;
+      res = kForkInvalid;
+    } else {
+      const int whole = (int)fastdiv((uint32_t)len, p.bs_div);
+      for (int j = threadIdx.x; j < n; j += kPgThreads) {
+        p.ws_pages[(int64_t)i * p.MB + j] = src[j];
+        if (j < whole) atomicAdd(p.refs + src[j], 1);
+      }
+      if (whole < n) last = src[whole];
+    }
+  }
+  if (threadIdx.x == 0) {
+    p.ws_len[i] = len;
+    p.ws_last[i] = last;
+    p.result[i] = res;
+  }
+}
+
+// Exclusive prefix sum over the work-group's kScan threads, and the total.
+__device__ inline int scan_block(int v, int& total, int* s_part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // (s_part of the last call has been read)
+  if (lane == 63) s_part[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kScan / 64; ++w) {
+    const int n = s_part[w];
+    before += w < wave ? n : 0;
+    total += n;
+  }
+  return before + x - v;
+}
+
+// One work-group.  A begun page that nobody holds any more goes to the lowest
+// entry forked from it; every other entry with a begun page gets a copy, in the
+// lowest free page, in the order of the entries.  Free pages are found in one
+// pass over the counts that ends when there are enough.
+__global__ __launch_bounds__(kScan) void fork_alloc_kernel(const ForkParams p) {
+  __shared__ int s_part[kScan / 64];
+  const int tid = threadIdx.x;
+  const int64_t NB = p.pool.num_blocks;
+  for (int i = tid; i < p.N; i += kScan) {
+    const int32_t last = p.ws_last[i];
+    if (last >= 0) atomicExch(p.ws_owner + last, INT32_MAX);
+  }
+  __syncthreads();
+  for (int i = tid; i < p.N; i += kScan) {
+    const int32_t last = p.ws_last[i];
+    if (last >= 0 && load_now(p.refs + last) == 0) atomicMin(p.ws_owner + last, i);
+  }
+  __syncthreads();
+  // Ranks of the entries that need a page, kept in ws_new until it is known.
+  int need = 0;
+  for (int i0 = 0; i0 < p.N; i0 += kScan) {
+    const int i = i0 + tid;
+    const int32_t last = i < p.N ? p.ws_last[i] : -1;
+    const bool takes = last >= 0 && load_now(p.ws_owner + last) == i;
+    const bool wants = last >= 0 && !takes;
+    int total;
+    const int rank = need + scan_block(wants ? 1 : 0, total, s_part);
+    if (i < p.N) p.ws_new[i] = wants ? rank : -1;
+    need += total;
+  }
+  __syncthreads();  // the owners have been read: their pages may be counted
+  for (int i = tid; i < p.N; i += kScan) {
+    const int32_t last = p.ws_last[i];
+    if (last >= 0 && p.ws_new[i] < 0) atomicExch(p.refs + last, 1);
+  }
+  __syncthreads();
+  // ws_owner's use is over: its first entries take the free pages.
+  int found = 0;
+  for (int64_t b0 = 0; b0 < NB && found < need; b0 += 4 * kScan) {
+    int32_t r[4];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t pg = b0 + 4 * tid + k;
+      r[k] = pg < NB ? load_now(p.refs + pg) : 1;
+      n += r[k] == 0;
+    }
+    int total;
+    int rank = found + scan_block(n, total, s_part);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (r[k] != 0) continue;
+      if (rank < need) atomicExch(p.ws_owner + rank, (int32_t)(b0 + 4 * tid + k));
+      ++rank;
+    }
+    found += total;
+  }
+  __syncthreads();
+  for (int i = tid; i < p.N; i += kScan) {
+    const int rank = p.ws_new[i];
+    if (rank < 0) continue;
+    if (rank < found) {
+      const int32_t pg = load_now(p.ws_owner + rank);
+      p.ws_new[i] = pg;
+      p.result[i] = pg;
+      atomicExch(p.refs + pg, 1);
+    } else {
+      p.ws_new[i] = -1;
+      p.result[i] = kForkNoPage;
+    }
+  }
+}
+
+// The first N work-groups write the rows (an entry without a page lets go of
+// what it shared and ends empty); the others copy the begun pages.
+__global__ __launch_bounds__(kPgThreads) void fork_write_kernel(const ForkParams p) {
+  if ((int)blockIdx.x < p.N) {
+    const int i = blockIdx.x;
+    int32_t len = p.ws_len[i];
+    if (len < 0) return;
+    const int32_t row = p.rows[i];
+    const int32_t* src = p.ws_pages + (int64_t)i * p.MB;
+    int32_t* dst = p.tables + row * p.tb_stride;
+    const int whole = (int)fastdiv((uint32_t)len, p.bs_div);
+    if (p.result[i] == kForkNoPage) {
+      for (int j = threadIdx.x; j < whole; j += kPgThreads) atomicAdd(p.refs + src[j], -1);
+      len = 0;
+    }
+    const int n = pages_of(p, len);
+    const int32_t fresh = p.ws_new[i];
+    for (int j = threadIdx.x; j < p.MB; j += kPgThreads)
+      dst[j] = j >= n ? -1 : j == whole && fresh >= 0 ? fresh : src[j];
+    if (threadIdx.x == 0) p.lens[row] = len;
+    return;
+  }
+  const uint32_t items = (uint32_t)page_items(p.pool);
+  const int64_t all = (int64_t)p.N * p.pool.planes * items;
+  for (int64_t x = (int64_t)blockIdx.x - p.N; x < all; x += (int64_t)gridDim.x - p.N) {
+    const int64_t y = x / items;
+    const int i = (int)(y / p.pool.planes);
+    const int32_t fresh = p.ws_len[i] < 0 ? -1 : p.ws_new[i];
+    if (fresh >= 0)
+      copy_item(p.pool, (int)(y - (int64_t)i * p.pool.planes), p.ws_last[i], fresh, (int)(x - y * items) * kPiece);
+  }
+}
+
+// Rows emptied without a cache or workspace: one launch.
+__global__ __launch_bounds__(kPgThreads) void free_kernel(const ForkParams p) {
+  const int i = blockIdx.x;
+  const int32_t row = p.rows[i];
+  if (!first_of_row(p.rows, i, row) || row < 0 || row >= p.R) return;
+  int32_t* t = p.tables + row * p.tb_stride;
+  const int held = pages_of(p, p.lens[row]);
+  __syncthreads();  // every thread has the length
+  for (int j = threadIdx.x; j < p.MB; j += kPgThreads) {
+    const int32_t pg = t[j];
+    if (j < held && pg >= 0 && pg < p.pool.num_blocks) atomicAdd(p.refs + pg, -1);
+    t[j] = -1;
+  }
+  if (threadIdx.x == 0) p.lens[row] = 0;
+}
+
+hipError_t launch_free(const ForkParams& p, hipStream_t stream) {
+  note_launch("pa::free_kernel");
+  hipLaunchKernelGGL(free_kernel, dim3(p.N), dim3(kPgThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_fork(const ForkParams& p, hipStream_t stream) {
+  note_launch("pa::fork_share_kernel");
+  hipLaunchKernelGGL(fork_share_kernel, dim3(p.N), dim3(kPgThreads), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  note_launch("pa::fork_alloc_kernel");
+  hipLaunchKernelGGL(fork_alloc_kernel, dim3(1), dim3(kScan), 0, stream, p);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const int64_t copies = std::min<int64_t>((int64_t)p.N * p.pool.planes * page_items(p.pool), kMaxGrid);
+  note_launch("pa::fork_write_kernel");
+  hipLaunchKernelGGL(fork_write_kernel, dim3((unsigned)(p.N + copies)), dim3(kPgThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- compact --
+// With n live pages, live page q >= n number j (ascending) moves to the free
+// page below n number j: as few moves as any dense order needs, and the pages
+// written (below n) are never read.
+
+constexpr int kCompactPer = kCompactPages / kPgThreads;  // consecutive pages of a thread
+
+__device__ inline int block_sum(int v, int* s_part) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if (lane == 0) s_part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return s_part[0] + s_part[1] + s_part[2] + s_part[3];
+}
+
+__global__ __launch_bounds__(kPgThreads) void compact_count_kernel(const CompactParams p) {
+  __shared__ int s_part[4];
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < kCompactPer; ++k) {
+    const int64_t pg = (int64_t)blockIdx.x * kCompactPages + k * kPgThreads + threadIdx.x;
+    n += pg < p.pool.num_blocks && p.refs[pg] > 0;
+  }
+  n = block_sum(n, s_part);
+  if (threadIdx.x == 0) p.ws_count[blockIdx.x] = n;
+}
+
+__global__ __launch_bounds__(kPgThreads) void compact_map_kernel(const CompactParams p) {
+  __shared__ int s_part[4];
+  const int tid = threadIdx.x;
+  const int64_t NB = p.pool.num_blocks;
+  // Live pages: in all, before this block, and before page `live` itself (the
+  // free pages among the first `live` are as many as the live ones after them).
+  int all = 0, mine = 0;
+  for (int b = tid; b < p.blocks; b += kPgThreads) {
+    const int c = p.ws_count[b];
+    all += c;
+    mine += b < (int)blockIdx.x ? c : 0;
+  }
+  all = block_sum(all, s_part);
+  mine = block_sum(mine, s_part);
+  const int cut = all / kCompactPages;  // the block that holds page `all`
+  int below = 0;
+  for (int b = tid; b < cut; b += kPgThreads) below += p.ws_count[b];
+  for (int k = tid; k < all - cut * kCompactPages; k += kPgThreads)
+    below += p.refs[(int64_t)cut * kCompactPages + k] > 0;
+  below = block_sum(below, s_part);
+
+  // This block's pages, kCompactPer consecutive ones per thread.
+  const int64_t first = (int64_t)blockIdx.x * kCompactPages + tid * kCompactPer;
+  int32_t r[kCompactPer];
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < kCompactPer; ++k) {
+    r[k] = first + k < NB ? p.refs[first + k] : 0;
+    n += r[k] > 0;
+  }
+  const int lane = tid & 63;
+  int x = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) s_part[tid >> 6] = x;
+  __syncthreads();
+  int before = mine + x - n;
+  for (int w = 0; w < (tid >> 6); ++w) before += s_part[w];
+#pragma unroll
+  for (int k = 0; k < kCompactPer; ++k) {
+    const int64_t pg = first + k;
+    if (pg >= NB) break;
+    const bool live = r[k] > 0;
+    if (pg < all) {
+      if (!live) p.ws_to[pg - before] = (int32_t)pg;
+      p.page_map[pg] = live ? (int32_t)pg : -1;
+      p.refs_out[pg] = r[k];
+    } else {
+      // A moved page's entry holds its number in the order of the moves, as -2 -
+      // number, until the move writes where it goes.
+      if (live) p.ws_from[before - below] = (int32_t)pg;
+      p.page_map[pg] = live ? -2 - (before - below) : -1;
+      p.refs_out[pg] = r[k];
+    }
+    before += live;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    p.ws_moves[0] = all - below;
+    p.num_live[0] = all;
+  }
+}
+
+// The moves, and the tables brought in line.  A table entry whose page's map
+// entry is being written meanwhile reads either form of it: the number leads to
+// the same place.
+__global__ __launch_bounds__(kPgThreads) void compact_move_kernel(const CompactParams p) {
+  const int moves = p.ws_moves[0];
+  const int64_t NB = p.pool.num_blocks, step = (int64_t)gridDim.x * kPgThreads;
+  const int64_t at = (int64_t)blockIdx.x * kPgThreads + threadIdx.x;
+  for (int64_t j = at; j < moves; j += step) {
+    const int32_t from = p.ws_from[j], to = p.ws_to[j];
+    const int32_t count = p.refs[from];
+    p.page_map[from] = to;
+    p.refs_out[to] = count;
+    p.refs_out[from] = 0;
+  }
+  for (int64_t e = at; e < (int64_t)p.R * p.MB; e += step) {
+    const int64_t row = e / p.MB, col = e - row * p.MB;
+    int32_t pg = p.tables[row * p.tb_stride + col];
+    if (pg >= 0 && pg < NB) {
+      pg = load_now(p.page_map + pg);
+      if (pg <= -2) pg = p.ws_to[-2 - pg];
+    }
+    p.tables_out[row * p.tbo_stride + col] = pg;
+  }
+  const uint32_t items = (uint32_t)page_items(p.pool);
+  const int64_t all = (int64_t)moves * p.pool.planes * items;
+  for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
+    const int64_t y = x / items;
+    const int j = (int)(y / p.pool.planes);
+    copy_item(p.pool, (int)(y - (int64_t)j * p.pool.planes), p.ws_from[j], p.ws_to[j], (int)(x - y * items) * kPiece);
+  }
+}
+
+hipError_t launch_compact(const CompactParams& p, hipStream_t stream) {
+  note_launch("pa::compact_count_kernel");
+  hipLaunchKernelGGL(compact_count_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  note_launch("pa::compact_map_kernel");
+  hipLaunchKernelGGL(compact_map_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  // At most half of the pages move.
+  const int64_t work = std::max<int64_t>((p.pool.num_blocks / 2 + 1) * p.pool.planes * page_items(p.pool),
+                                         (int64_t)p.R * p.MB / kPgThreads + 1);
+  note_launch("pa::compact_move_kernel");
+  hipLaunchKernelGGL(compact_move_kernel, dim3((unsigned)std::min<int64_t>(work, 2048)), dim3(kPgThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace pa

@@ -264,6 +264,91 @@ void op_write_kv_into(const at::Tensor& k_cache, const at::Tensor& v_cache, cons
   op_write_kv_scaled(k, v, key, value, slot_mapping, k_scale, v_scale);
 }
 
+// ------------------------------------------- norm, rotation and write; pages --
+
+// A view or nothing.
+struct OptView {
+  pa_tensor_t t;
+  bool have = false;
+  explicit OptView(const std::optional<at::Tensor>& x) {
+    if (x.has_value()) {
+      t = view(*x);
+      have = true;
+    }
+  }
+  pa_tensor_t* get() { return have ? &t : nullptr; }
+};
+
+void one_device(const at::Tensor& q, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* t : others)
+    TORCH_CHECK(t->device() == q.device(), "all tensors must be on one device");
+}
+
+void op_qk_norm_rope_write_kv_out(const at::Tensor& q, const at::Tensor& key, const at::Tensor& value,
+                                  const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                  const at::Tensor& slot_mapping, const at::Tensor& cos_sin,
+                                  const at::Tensor& positions, const std::optional<at::Tensor>& q_weight,
+                                  const std::optional<at::Tensor>& k_weight, double eps, bool interleaved,
+                                  double k_scale, double v_scale, const at::Tensor& out) {
+  one_device(q, {&key, &value, &k_cache, &v_cache, &slot_mapping, &cos_sin, &positions, &out});
+  for (const auto* w : {&q_weight, &k_weight})
+    if (w->has_value()) one_device(q, {&**w});
+  c10::DeviceGuard guard(q.device());
+  pa_tensor_t o = view(out), kc = view(k_cache), vc = view(v_cache), qq = view(q), kk = view(key), vv = view(value),
+              ss = view(slot_mapping), cs = view(cos_sin), pp = view(positions);
+  OptView qw(q_weight), kw(k_weight);
+  check(pa_qk_norm_rope_write_kv(&o, &kc, &vc, &qq, &kk, &vv, &ss, &cs, &pp, qw.get(), kw.get(), eps,
+                                 interleaved ? 1 : 0, k_scale, v_scale, stream_of(q)));
+}
+
+void op_copy_pages(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache, const at::Tensor& src,
+                   const at::Tensor& dst) {
+  one_device(k_cache, {&src, &dst});
+  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  c10::DeviceGuard guard(k_cache.device());
+  pa_tensor_t k = view(k_cache), s = view(src), d = view(dst);
+  OptView v(v_cache);
+  check(pa_copy_pages(&k, v.get(), &s, &d, stream_of(k_cache)));
+}
+
+at::Tensor op_fork_sequences(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache,
+                             const at::Tensor& block_tables, const at::Tensor& context_lens,
+                             const at::Tensor& page_refs, const at::Tensor& parents, const at::Tensor& rows) {
+  one_device(k_cache, {&block_tables, &context_lens, &page_refs, &parents, &rows});
+  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  c10::DeviceGuard guard(k_cache.device());
+  at::Tensor copied = at::empty(rows.sizes(), rows.options());
+  pa_tensor_t k = view(k_cache), bt = view(block_tables), cl = view(context_lens), rf = view(page_refs),
+              pr = view(parents), rw = view(rows), cp = view(copied);
+  OptView v(v_cache);
+  Scratch s = scratch_of(k_cache, pa_fork_workspace_size(&bt, &rf, &rw));
+  check(pa_fork_sequences(&k, v.get(), &bt, &cl, &rf, &pr, &rw, &cp, s.ptr, s.bytes, stream_of(k_cache)));
+  return copied;
+}
+
+void op_free_sequences(const at::Tensor& block_tables, const at::Tensor& context_lens, const at::Tensor& page_refs,
+                       const at::Tensor& rows, int64_t block_size) {
+  one_device(block_tables, {&context_lens, &page_refs, &rows});
+  c10::DeviceGuard guard(block_tables.device());
+  pa_tensor_t bt = view(block_tables), cl = view(context_lens), rf = view(page_refs), rw = view(rows);
+  check(pa_free_sequences(&bt, &cl, &rf, &rw, block_size, stream_of(block_tables)));
+}
+
+std::tuple<at::Tensor, at::Tensor> op_compact_pages(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache,
+                                                    const at::Tensor& block_tables, const at::Tensor& page_refs,
+                                                    const at::Tensor& tables_out, const at::Tensor& refs_out) {
+  one_device(k_cache, {&block_tables, &page_refs, &tables_out, &refs_out});
+  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  c10::DeviceGuard guard(k_cache.device());
+  at::Tensor map = at::empty(page_refs.sizes(), page_refs.options()), n = at::empty({1}, page_refs.options());
+  pa_tensor_t k = view(k_cache), bt = view(block_tables), rf = view(page_refs), to = view(tables_out),
+              ro = view(refs_out), mp = view(map), nl = view(n);
+  OptView v(v_cache);
+  Scratch s = scratch_of(k_cache, pa_compact_workspace_size(&rf));
+  check(pa_compact_pages(&k, v.get(), &bt, &rf, &to, &ro, &mp, &nl, s.ptr, s.bytes, stream_of(k_cache)));
+  return {map, n};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(gb10_attn, m) {
@@ -302,6 +387,16 @@ TORCH_LIBRARY(gb10_attn, m) {
   m.def("write_kv_scaled(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor key, Tensor value, Tensor slot_mapping, "
         "float k_scale, float v_scale) -> ()",
         &op_write_kv_scaled);
+  m.def("qk_norm_rope_write_kv_out(Tensor q, Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+        "Tensor slot_mapping, Tensor cos_sin, Tensor positions, Tensor? q_weight, Tensor? k_weight, float eps, "
+        "bool interleaved, float k_scale, float v_scale, Tensor(c!) out) -> ()");
+  m.def("copy_pages(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor src, Tensor dst) -> ()");
+  m.def("fork_sequences(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor(c!) block_tables, Tensor(d!) context_lens, "
+        "Tensor(e!) page_refs, Tensor parents, Tensor rows) -> Tensor");
+  m.def("free_sequences(Tensor(a!) block_tables, Tensor(b!) context_lens, Tensor(c!) page_refs, Tensor rows, "
+        "int block_size) -> ()");
+  m.def("compact_pages(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor block_tables, Tensor page_refs, "
+        "Tensor(c!) tables_out, Tensor(d!) refs_out) -> (Tensor, Tensor)");
 }
 
 // The Python functions' operators have a GPU kernel only: under torch.compile
@@ -310,4 +405,9 @@ TORCH_LIBRARY_IMPL(gb10_attn, CUDA, m) {
   m.impl("decode_out", &op_decode_out);
   m.impl("prefill_out", &op_prefill_out);
   m.impl("write_kv_into", &op_write_kv_into);
+  m.impl("qk_norm_rope_write_kv_out", &op_qk_norm_rope_write_kv_out);
+  m.impl("copy_pages", &op_copy_pages);
+  m.impl("fork_sequences", &op_fork_sequences);
+  m.impl("free_sequences", &op_free_sequences);
+  m.impl("compact_pages", &op_compact_pages);
 }

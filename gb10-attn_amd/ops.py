@@ -127,6 +127,48 @@ class _CAbi:
             check(lib().pa_write_kv_scaled(*(C.byref(view(t)) for t in (k_cache, v_cache, key, value, slot_mapping)),
                                            k_scale, v_scale, _stream(key.device)))
 
+    @staticmethod
+    def qk_norm_rope_write_kv_out(q, key, value, k_cache, v_cache, slot_mapping, cos_sin, positions, q_weight, k_weight,
+                                  eps, interleaved, k_scale, v_scale, out):
+        with torch.cuda.device(q.device):
+            check(lib().pa_qk_norm_rope_write_kv(*_refs(out, k_cache, v_cache, q, key, value, slot_mapping, cos_sin,
+                                                        positions, q_weight, k_weight), eps, int(interleaved), k_scale,
+                                                 v_scale, _stream(q.device)))
+
+    @staticmethod
+    def copy_pages(k_cache, v_cache, src, dst):
+        with torch.cuda.device(k_cache.device):
+            check(lib().pa_copy_pages(*_refs(k_cache, v_cache, src, dst), _stream(k_cache.device)))
+
+    @staticmethod
+    def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows):
+        copied = torch.empty(rows.shape, dtype=torch.int32, device=rows.device)
+        with torch.cuda.device(rows.device):
+            ws = _scratch(lib().pa_fork_workspace_size(*_refs(block_tables, page_refs, rows)), rows.device)
+            check(lib().pa_fork_sequences(*_refs(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows,
+                                                 copied), ws.data_ptr(), ws.numel(), _stream(rows.device)))
+        return copied
+
+    @staticmethod
+    def free_sequences(block_tables, context_lens, page_refs, rows, block_size):
+        with torch.cuda.device(rows.device):
+            check(lib().pa_free_sequences(*_refs(block_tables, context_lens, page_refs, rows), block_size,
+                                          _stream(rows.device)))
+
+    @staticmethod
+    def compact_pages(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out):
+        dev = page_refs.device
+        page_map, n = torch.empty_like(page_refs), torch.empty(1, dtype=torch.int32, device=dev)
+        with torch.cuda.device(dev):
+            ws = _scratch(lib().pa_compact_workspace_size(*_refs(page_refs)), dev)
+            check(lib().pa_compact_pages(*_refs(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out,
+                                                page_map, n), ws.data_ptr(), ws.numel(), _stream(dev)))
+        return page_map, n
+
+
+def _refs(*tensors):
+    return [None if t is None else C.byref(view(t)) for t in tensors]
+
 
 def _native():
     if _ops is None and not _torch_path().exists():
@@ -277,6 +319,112 @@ def write_kv_blocks(kv_pool, block_ids, start, k, v, k_scale=1.0, v_scale=1.0):
     for layer in range(L):
         write_kv(kv_pool[layer, 0], kv_pool[layer, 1], k[layer].permute(1, 0, 2), v[layer].permute(1, 0, 2), slots,
                  k_scale, v_scale)
+
+
+def qk_norm_rope_write_kv(q, key, value, k_cache, v_cache, slot_mapping, cos_sin, positions, *, q_weight=None,
+                          k_weight=None, eps=1e-6, interleaved=False, k_scale=1.0, v_scale=1.0, out_dtype=None,
+                          out=None):
+    """Norm and rotation of new heads with the KV-cache write, in one pass (pa_qk_norm_rope_write_kv).
+
+    q [T, H, D] and key/value [T, HKV, D] (fp32/fp16/bf16; views of a packed
+    projection are read in place).  Each q and key head is divided by its root mean
+    square and multiplied by q_weight / k_weight [D] (None: no norm), then rotated
+    by the cosines and sines of its token's row of cos_sin [positions, rot] (cosines
+    first; rot <= D, the rest passes): pairs (i, i + rot/2), or neighbours with
+    interleaved=True.  Keys and values go to k_cache/v_cache at slot_mapping as
+    write_kv writes them; returns the queries (a new tensor of q's type, out_dtype,
+    or `out`, which may be q)."""
+    for t, n in ((q, "q"), (key, "key"), (value, "value"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must be on CUDA")
+    if q.dim() != 3 or key.dim() != 3 or value.dim() != 3:
+        raise RuntimeError("q must be [T, H, D], key/value [T, HKV, D]")
+    if not _kv_ok(k_cache) or not _kv_ok(v_cache):
+        raise RuntimeError("k_cache/v_cache must be 16-byte aligned [NB, BS, HKV, D] views with a contiguous last dim")
+    o = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device) if out is None else out
+    q, key, value, cos_sin = (_rows(t) for t in (q, key, value, cos_sin))
+    q_weight, k_weight = (t if t is None else _rows(t) for t in (q_weight, k_weight))
+    _native().qk_norm_rope_write_kv_out(q, key, value, k_cache, v_cache, _index(slot_mapping, q.device), cos_sin,
+                                        _index(positions, q.device), q_weight, k_weight, float(eps), bool(interleaved),
+                                        float(k_scale), float(v_scale), o)
+    return o
+
+
+def _rows(t):
+    """t, or a copy where the row kernels cannot read it in place (last dimension, alignment)."""
+    es = t.element_size()
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        t.stride(i) >= 0 and (t.stride(i) * es % 16 == 0 or t.shape[i] == 1) for i in range(t.dim() - 1))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _index(t, dev):
+    if t.dtype not in (torch.int32, torch.int64):
+        t = t.to(torch.int64)
+    return t.to(dev).contiguous()
+
+
+def _pages(t):
+    """A cache [NB, BS, HKV, D] or [L, NB, BS, HKV, D] (one layer or all of them: e.g. kv_pool[:, 0]) as
+    [L, NB, BS, HKV * D]."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise RuntimeError("kv cache must be on CUDA")
+    if t.dim() not in (4, 5):
+        raise RuntimeError("k_cache/v_cache must be [NB, BS, HKV, D] or [L, NB, BS, HKV, D]")
+    t = t if t.dim() == 5 else t[None]
+    L, NB, BS, HKV, D = t.shape
+    if (D > 1 and t.stride(4) != 1) or (HKV > 1 and t.stride(3) != D):
+        raise RuntimeError("k_cache/v_cache must have contiguous token rows")
+    return t.as_strided((L, NB, BS, HKV * D), (*t.stride()[:3], 1))
+
+
+def _state(*tensors):
+    """Block tables, lengths and counts are updated in place: int32 on the GPU."""
+    for t in tensors:
+        if t.dtype != torch.int32 or not t.is_cuda:
+            raise RuntimeError("block_tables, context_lens and page_refs must be int32 on CUDA")
+
+
+def copy_pages(k_cache, v_cache, src, dst):
+    """Pages src[i] -> dst[i] of a cache ([NB, BS, HKV, D], or [L, NB, BS, HKV, D] for every layer at once;
+    v_cache may be None) in one launch.  Negative or outside pages are skipped; a destination named
+    twice takes the last pair that names it (pa_copy_pages).  In place; returns nothing."""
+    k = _pages(k_cache)
+    _native().copy_pages(k, _pages(v_cache), *(t.to(k.device, torch.int32).contiguous() for t in (src, dst)))
+
+
+def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows):
+    """Rows of the block tables become forks of others: row rows[i] lets go of its pages and shares
+    those of row parents[i], whose begun page is copied to the lowest free page unless no row
+    would hold it any more; a negative parent empties the row (pa_fork_sequences, which also says
+    what happens to entries that cannot be served).  Parents are read as the call finds them, so a
+    beam step may permute and branch rows in place.  block_tables [R, MB], context_lens [R] and
+    page_refs [NB] (holders per page, 0 = free) are int32 and updated in place.  Returns int32 [N]:
+    the page each begun page was copied to, -1 none needed, -2 no page free, -3 refused."""
+    _state(block_tables, context_lens, page_refs)
+    dev = block_tables.device
+    return _native().fork_sequences(_pages(k_cache), _pages(v_cache), block_tables, context_lens, page_refs,
+                                    parents.to(dev, torch.int32).contiguous(), rows.to(dev, torch.int32).contiguous())
+
+
+def free_sequences(block_tables, context_lens, page_refs, rows, block_size):
+    """Rows of the block tables let go of their pages and end empty, in place (pa_free_sequences)."""
+    _state(block_tables, context_lens, page_refs)
+    _native().free_sequences(block_tables, context_lens, page_refs,
+                             rows.to(block_tables.device, torch.int32).contiguous(), int(block_size))
+
+
+def compact_pages(k_cache, v_cache, block_tables, page_refs, *, tables_out=None, refs_out=None):
+    """Moves the pages in use (page_refs > 0) to the front of the cache, in every layer, with as few moves
+    as a dense cache allows, and brings block_tables and page_refs in line: in place, or into
+    tables_out / refs_out (pa_compact_pages).  Returns (page_map [NB]: each page's place now, -1 for
+    a free one; num_live [1]), int32 on the GPU."""
+    tables_out = block_tables if tables_out is None else tables_out
+    refs_out = page_refs if refs_out is None else refs_out
+    _state(block_tables, page_refs, tables_out, refs_out)
+    return _native().compact_pages(_pages(k_cache), _pages(v_cache), block_tables, page_refs, tables_out, refs_out)
 
 
 _ops = None

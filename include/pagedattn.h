@@ -329,6 +329,84 @@ int pa_write_kv_scaled(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tens
                        const pa_tensor_t* value, const pa_tensor_t* slot_mapping, double k_scale,
                        double v_scale, void* stream);
 
+/* New queries and keys on their way into the paged cache: the RMS norm of each
+ * head, the rotation by position and pa_write_kv_scaled's write in one pass.
+ *   y = x * rsqrt(mean(x^2) + eps) * weight    over each head's D elements, where
+ *       q_weight / k_weight ([D], float32, float16 or bfloat16) is not NULL;
+ *   (a, b) -> (a cos - b sin, b cos + a sin)   over the first rot elements: pairs
+ *       (i, i + rot/2), or (2i, 2i + 1) with interleaved != 0; cos and sin of pair
+ *       i are cos_sin[n][i] and cos_sin[n][rot/2 + i] at the token's position n.
+ * q [T, H, D] and key/value [T, HKV, D] share a type (float32, float16, bfloat16)
+ * and may be views of one packed projection (last dimension contiguous, 16-byte
+ * aligned strides); q_out [T, H, D] of any of these types receives the queries (it
+ * may be q itself), k_cache / v_cache the keys and values at slot_mapping, divided
+ * by their scales, as pa_write_kv_scaled.  cos_sin [positions, rot], rot a multiple
+ * of 16 (rot <= D; D a multiple of 16 up to 256), float32, float16 or bfloat16;
+ * positions and slot_mapping int32 or int64 [T].  Arithmetic is fp32, each result
+ * rounded once.  A negative slot (padding), or one past the pool, writes nothing; a
+ * position outside the table makes the rotated elements NaN.  Tokens of one call
+ * need slots of their own.  No reference counterpart (the reference's engine
+ * writes finished keys, harness/repro_crash.py:52-58). */
+int pa_qk_norm_rope_write_kv(pa_tensor_t* q_out, pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* q,
+                             const pa_tensor_t* key, const pa_tensor_t* value, const pa_tensor_t* slot_mapping,
+                             const pa_tensor_t* cos_sin, const pa_tensor_t* positions, const pa_tensor_t* q_weight,
+                             const pa_tensor_t* k_weight, double eps, int interleaved, double k_scale,
+                             double v_scale, void* stream);
+
+/* Pages of a cache copied, shared and made dense.  Here a cache is [L, NB, BS, row]
+ * (L layers, or 1; row = HKV * D elements, contiguous; any type; strides multiples
+ * of 16 bytes), K and V of the same shape, v_cache NULL where there is one cache
+ * only.  Sequences are rows of block_tables (int32 [R, MB]) with context_lens
+ * (int32 [R]); page_refs (int32 [NB]) counts the rows that hold each page, 0 for a
+ * free page.  All of it is device memory, updated in stream order; nothing
+ * synchronises.  The reference leaves its pages to an engine outside it
+ * (harness/repro_crash.py:52-58). */
+
+/* Pages src[i] -> dst[i] (int32 [N]) of every layer.  Pairs with a page outside the
+ * pool are skipped; a destination named twice takes the last pair that names it.
+ * A page that is both a source and a destination has unspecified contents in the
+ * pages copied from it. */
+int pa_copy_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* src, const pa_tensor_t* dst,
+                  void* stream);
+
+/* For each i in order, row rows[i] lets go of its pages and becomes a fork of row
+ * parents[i] as the call found it: the parent's whole pages are shared, a page it
+ * has begun is copied to the lowest-numbered free page (in the order of the
+ * entries), unless after the call no row would hold it, when the lowest such entry
+ * keeps it.  A row may be a parent and be replaced in one call (beam steps).  A
+ * negative parent, or parents NULL, empties the row.  Entries past a row's pages
+ * are set to -1.  copied[i] (int32 [N]) is the page a begun page was copied to, or
+ *   -1: no copy was needed;
+ *   -2: no page was free: the row ends empty;
+ *   -3: the entry was refused: a row outside [0, R) or named before (nothing is
+ *       done), or a parent >= R, longer than its table or with a page outside the
+ *       pool (the row ends empty).
+ * At most 65536 entries.  workspace: device memory of
+ * pa_fork_workspace_size(...) bytes, 256-byte aligned, of this call alone. */
+int pa_fork_sequences(pa_tensor_t* k_cache, pa_tensor_t* v_cache, pa_tensor_t* block_tables,
+                      pa_tensor_t* context_lens, pa_tensor_t* page_refs, const pa_tensor_t* parents,
+                      const pa_tensor_t* rows, pa_tensor_t* copied, void* workspace, size_t workspace_bytes,
+                      void* stream);
+size_t pa_fork_workspace_size(const pa_tensor_t* block_tables, const pa_tensor_t* page_refs, const pa_tensor_t* rows);
+
+/* The rows let go of their pages and end empty (one launch, no workspace). */
+int pa_free_sequences(pa_tensor_t* block_tables, pa_tensor_t* context_lens, pa_tensor_t* page_refs,
+                      const pa_tensor_t* rows, int64_t block_size, void* stream);
+
+/* Makes the pages in use dense.  With n pages of count > 0, the j-th of them at or
+ * past n (ascending) moves to the j-th free page below n, in every layer; pages
+ * below n stay.  tables_out and refs_out (which may be block_tables and page_refs
+ * themselves, or else must not overlap them) receive the updated state: every entry
+ * that names a moved page names its new place, one that names a free page becomes
+ * -1, others are as they were.  page_map (int32 [NB]): where each page in use is
+ * now, -1 for a free one; num_live (int32 [1]): n.  A moved page's old place keeps
+ * its contents.  workspace: pa_compact_workspace_size(...) bytes, as above. */
+int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* block_tables,
+                     const pa_tensor_t* page_refs, pa_tensor_t* tables_out, pa_tensor_t* refs_out,
+                     pa_tensor_t* page_map, pa_tensor_t* num_live, void* workspace, size_t workspace_bytes,
+                     void* stream);
+size_t pa_compact_workspace_size(const pa_tensor_t* page_refs);
+
 #ifdef __cplusplus
 }
 #endif
