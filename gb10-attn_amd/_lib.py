@@ -32,6 +32,7 @@ EXPORTS = (
     "pa_write_kv", "pa_write_kv_scaled", "pa_qk_norm_rope_write_kv",
     "pa_copy_pages", "pa_fork_sequences", "pa_fork_workspace_size", "pa_free_sequences",
     "pa_compact_pages", "pa_compact_workspace_size",
+    "paged_attention_shared_prefix", "paged_attention_shared_prefix_workspace_size",
 )
 
 
@@ -129,6 +130,10 @@ def lib() -> C.CDLL:
     L.pa_compact_pages.argtypes = [T] * 8 + [P, sz, P]
     L.pa_compact_workspace_size.restype = sz
     L.pa_compact_workspace_size.argtypes = [T]
+    L.paged_attention_shared_prefix.restype = C.c_int
+    L.paged_attention_shared_prefix.argtypes = [T] * 8 + [C.c_double] * 3 + [P, sz, P]
+    L.paged_attention_shared_prefix_workspace_size.restype = sz
+    L.paged_attention_shared_prefix_workspace_size.argtypes = [T] * 4
     _lib = L
     return L
 

@@ -47,6 +47,19 @@ hipError_t launch_decode_f32(const DecodeParams& p, int gc, hipStream_t stream);
 hipError_t launch_decode_f64(const DecodeParams& p, int gc, hipStream_t stream);
 hipError_t launch_decode_fp8(const DecodeParams& p, int gc, hipStream_t stream);
 
+hipError_t launch_shared_f16(const SharedParams& p, hipStream_t stream);
+hipError_t launch_shared_bf16(const SharedParams& p, hipStream_t stream);
+hipError_t launch_shared_fp8(const SharedParams& p, hipStream_t stream);
+
+hipError_t launch_shared(const SharedParams& p, int kv_dtype, hipStream_t stream) {
+  switch (kv_dtype) {
+    case kF16: return launch_shared_f16(p, stream);
+    case kBF16: return launch_shared_bf16(p, stream);
+    case kFP8: return launch_shared_fp8(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 hipError_t launch_decode(const DecodeParams& p, int kv_dtype, int gc, hipStream_t stream) {
   switch (kv_dtype) {
     case kF16: return launch_decode_f16(p, gc, stream);
@@ -1564,4 +1577,133 @@ extern "C" int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, cons
   p.ws_count = p.ws_to + NB;
   p.ws_moves = p.ws_count + p.blocks;
   return hip_status(launch_compact(p, static_cast<hipStream_t>(stream)), "compaction kernel launch");
+}
+
+// ---------------------------------------------------------- shared prefixes --
+
+// Sizes and grid of a shared-prefix call.  The grid fills the GPU (two work-groups
+// per CU, one at D = 256), or has as many as the keys that the tables can hold make
+// shares of.
+static int plan_shared(SharedParams* p) {
+  int cus = 0, rc;
+  if ((rc = device_cu_count(&cus))) return rc;
+  if (p->B > kSharedMaxSeqs || p->NG > kSharedMaxSeqs)
+    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups", kSharedMaxSeqs);
+  const int64_t sg = (int64_t)p->S * p->G, rows = p->B * sg;
+  if (rows >= (1LL << 30)) return fail(PA_ERR_UNSUPPORTED, "too many query rows");
+  p->SG = (int32_t)sg;
+  p->own_rb = (int32_t)((sg + kSharedWide - 1) / kSharedWide);
+  p->cost_thin = 1;
+  p->cost_wide = 1;
+  p->min_share = 4;
+  const int64_t tiles = ((int64_t)p->MB * p->BS + kSharedTile - 1) / kSharedTile + 1;
+  const int64_t units = p->HKV * (rows / kSharedWide + p->NG + (int64_t)p->B * p->own_rb);
+  const int64_t most = units * tiles * std::max(p->cost_thin, p->cost_wide);
+  if (units >= (1LL << 31) || most >= (1LL << 31)) return fail(PA_ERR_UNSUPPORTED, "too many keys and query rows for one call");
+  p->wgs = (int32_t)std::min<int64_t>((p->D <= 128 ? 2 : 1) * (int64_t)cus, std::max<int64_t>(1, (most + p->min_share - 1) / p->min_share));
+  p->sg_div = make_fastdiv((uint32_t)std::max(1, p->SG));
+  p->g_div = make_fastdiv((uint32_t)std::max(1, p->G));
+  return PA_OK;
+}
+
+static size_t shared_meta_bytes(const SharedParams& p) { return (4 * (size_t)(3 + p.NG + p.B) + 255) & ~(size_t)255; }
+static size_t shared_rows(const SharedParams& p) {
+  const size_t own = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
+  return (size_t)p.wgs * (kSharedWide + own) + 2 * (size_t)p.HKV * p.B * p.SG;
+}
+static size_t shared_bytes(const SharedParams& p) { return shared_meta_bytes(p) + shared_rows(p) * (p.D + 2) * 4; }
+
+extern "C" size_t paged_attention_shared_prefix_workspace_size(const pa_tensor_t* q, const pa_tensor_t* k_cache,
+                                                               const pa_tensor_t* block_tables,
+                                                               const pa_tensor_t* group_starts) {
+  if (!q || (q->ndim != 3 && q->ndim != 4)) {
+    fail(PA_ERR_INVALID_ARGUMENT, "q must be [B, H, D] or [B, S, H, D]");
+    return (size_t)-1;
+  }
+  if (check_tensor(q, "q", q->ndim, "[B, S, H, D]") || check_tensor(k_cache, "k_cache", 4, "[NB, BS, H, D]") ||
+      check_tables(block_tables, "block_tables") || check_index(group_starts, "group_starts", -1, false))
+    return (size_t)-1;
+  const int64_t H = q->shape[q->ndim - 2], HKV = k_cache->shape[2], D = q->shape[q->ndim - 1];
+  const int64_t S = q->ndim == 4 ? q->shape[1] : 1;
+  if (HKV <= 0 || H <= 0 || H % HKV || k_cache->shape[1] <= 0 || H >= (1 << 16) || D <= 0 || D > 256) {
+    fail(PA_ERR_INVALID_ARGUMENT, "n_head must be divisible by n_kv_head, block_size positive and head_dim at most 256");
+    return (size_t)-1;
+  }
+  if (group_starts->shape[0] < 1) {
+    fail(PA_ERR_INVALID_ARGUMENT, "group_starts must have at least one entry");
+    return (size_t)-1;
+  }
+  if (q->shape[0] > kSharedMaxSeqs || S >= (1LL << 31) || group_starts->shape[0] > kSharedMaxSeqs + 1 ||
+      k_cache->shape[1] >= (1LL << 31) || block_tables->shape[1] * k_cache->shape[1] >= (1LL << 31)) {
+    fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups, and 32-bit token indices", kSharedMaxSeqs);
+    return (size_t)-1;
+  }
+  SharedParams p;
+  memset(&p, 0, sizeof(p));
+  p.B = (int32_t)q->shape[0]; p.S = (int32_t)S; p.H = (int32_t)H; p.HKV = (int32_t)HKV; p.G = (int32_t)(H / HKV);
+  p.D = (int32_t)D; p.BS = (int32_t)k_cache->shape[1]; p.MB = (int32_t)block_tables->shape[1];
+  p.NG = (int32_t)(group_starts->shape[0] - 1);
+  if (numel(q) == 0) return 0;
+  if (plan_shared(&p)) return (size_t)-1;
+  return shared_bytes(p);
+}
+
+extern "C" int paged_attention_shared_prefix(pa_tensor_t* out, const pa_tensor_t* q, const pa_tensor_t* k_cache,
+                                             const pa_tensor_t* v_cache, const pa_tensor_t* block_tables,
+                                             const pa_tensor_t* context_lens, const pa_tensor_t* group_starts,
+                                             const pa_tensor_t* prefix_lens, double scale, double k_scale,
+                                             double v_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  g_launches.clear();
+  if (!q || (q->ndim != 3 && q->ndim != 4))
+    return fail(PA_ERR_INVALID_ARGUMENT, "q must be [B, H, D] or [B, S, H, D]");
+  int rc;
+  if ((rc = check_tensor(out, "out", q->ndim, q->ndim == 3 ? "[B, H, D]" : "[B, S, H, D]"))) return rc;
+  if (!finite_f32(k_scale) || !finite_f32(v_scale))
+    return fail(PA_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be finite");
+  if (!finite_f32(scale * k_scale * 1.4426950408889634))
+    return fail(PA_ERR_INVALID_ARGUMENT, "scale * k_scale must be finite");
+  pa_tensor_t q4 = *q, o4 = *out;
+  if (q->ndim == 3) {
+    for (pa_tensor_t* t : {&q4, &o4}) {
+      t->ndim = 4;
+      t->shape[3] = t->shape[2]; t->shape[2] = t->shape[1]; t->shape[1] = 1;
+      t->stride[3] = t->stride[2]; t->stride[2] = t->stride[1]; t->stride[1] = t->shape[2] * t->shape[3];
+    }
+  }
+  DecodeArgs a;
+  if ((rc = check_args(&o4, &q4, k_cache, v_cache, block_tables, context_lens, scale * k_scale, true, &a))) return rc;
+  if (!prefill_kv(a.kv_dtype))
+    return fail(PA_ERR_INVALID_ARGUMENT, "shared prefixes need an fp16, bf16 or float8_e4m3fn KV cache");
+  if ((rc = check_index(group_starts, "group_starts", -1, false))) return rc;
+  if (group_starts->shape[0] < 1) return fail(PA_ERR_INVALID_ARGUMENT, "group_starts must have at least one entry");
+  if ((rc = check_index(prefix_lens, "prefix_lens", group_starts->shape[0] - 1, false))) return rc;
+  if (group_starts->shape[0] > kSharedMaxSeqs + 1)
+    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups", kSharedMaxSeqs);
+  const DecodeParams& d = a.p;
+  if ((int64_t)d.B * d.Sq * d.H == 0) return PA_OK;
+  if (!aligned16(q->data)) return fail(PA_ERR_UNSUPPORTED, "shared prefixes need a 16-byte aligned q");
+  SharedParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = d.q; p.out = d.out; p.k = d.k; p.v = d.v;
+  p.block_tables = d.block_tables; p.context_lens = d.context_lens;
+  p.group_starts = static_cast<const int32_t*>(group_starts->data);
+  p.prefix_lens = static_cast<const int32_t*>(prefix_lens->data);
+  p.k_sb = d.k_sb; p.k_st = d.k_st; p.k_sh = d.k_sh;
+  p.v_sb = d.v_sb; p.v_st = d.v_st; p.v_sh = d.v_sh;
+  p.bt_stride = d.bt_stride; p.num_blocks = d.num_blocks;
+  p.B = d.B; p.S = d.Sq; p.H = d.H; p.HKV = d.HKV; p.G = d.G; p.D = d.D; p.BS = d.BS; p.MB = d.MB;
+  p.NG = (int32_t)(group_starts->shape[0] - 1);
+  p.q_dtype = d.q_dtype; p.out_dtype = d.out_dtype;
+  p.bs_div = d.bs_div;
+  p.qscale = (float)(scale * k_scale * 1.4426950408889634);
+  p.vscale = (float)v_scale;
+  if ((rc = plan_shared(&p))) return rc;
+  if ((rc = check_scratch(shared_bytes(p), workspace, workspace_bytes))) return rc;
+  p.ws_meta = static_cast<int32_t*>(workspace);
+  p.ws_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + shared_meta_bytes(p));
+  p.ws_m = p.ws_acc + shared_rows(p) * p.D;
+  p.ws_l = p.ws_m + shared_rows(p);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if ((rc = hip_status(launch_shared(p, a.kv_dtype, s), "shared-prefix kernel launch"))) return rc;
+  return hip_status(launch_shared_merge(p, s), "shared-prefix merge kernel launch");
 }

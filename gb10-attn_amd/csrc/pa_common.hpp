@@ -302,6 +302,37 @@ struct CompactParams {
 };
 constexpr int kCompactPages = 2048;  // pages per work-group of the counting passes
 
+// Attention of groups of sequences that share a prefix.
+struct SharedParams {
+  const void* q;  // [B, S, H, D]
+  void* out;
+  const void* k;
+  const void* v;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  const int32_t* group_starts;  // [NG + 1]
+  const int32_t* prefix_lens;   // [NG]
+  int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh, bt_stride, num_blocks;
+  int32_t B, S, H, HKV, G, D, BS, MB, NG;
+  int32_t SG;      // S * G: query rows of a sequence under one KV head
+  int32_t own_rb;  // row blocks of a sequence's own keys
+  int32_t q_dtype, out_dtype;
+  int32_t wgs;               // work-groups of the grid
+  int32_t cost_thin, cost_wide;  // of a tile of keys, in the units that are shared out
+  int32_t min_share;         // fewest units of a work-group
+  FastDiv bs_div, sg_div, g_div;
+  float qscale, vscale;
+  // Workspace: share, fault and the cost sums; the pieces' softmax states.
+  int32_t* ws_meta;  // [2 + NG + 1 + B + 1]
+  float* ws_acc;     // [rows][D]
+  float* ws_m;       // [rows] log2 units
+  float* ws_l;       // [rows]
+};
+constexpr int kSharedWide = 128;  // query rows of a wide unit
+constexpr int kSharedThin = 16;   // ... of a thin one
+constexpr int kSharedTile = 64;   // keys of a tile
+constexpr int kSharedMaxSeqs = 1024;
+
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = 64 * kDecodeWaves;
 constexpr int kBtChunk = 256;  // block-table entries a decode work-group stages in LDS at a time
@@ -328,6 +359,8 @@ hipError_t launch_copy_pages(const CopyParams& p, hipStream_t stream);
 hipError_t launch_fork(const ForkParams& p, hipStream_t stream);
 hipError_t launch_free(const ForkParams& p, hipStream_t stream);
 hipError_t launch_compact(const CompactParams& p, hipStream_t stream);
+hipError_t launch_shared(const SharedParams& p, int kv_dtype, hipStream_t stream);
+hipError_t launch_shared_merge(const SharedParams& p, hipStream_t stream);
 
 // Head packing (heads contiguous in the pool; MHA, or GQA groups of four over
 // 16-bit caches): one decode work-group

@@ -1,0 +1,126 @@
+// pa_shared_merge.hip -- joins the states of a shared-prefix call (pa_shared.hpp) into
+// the output rows:
+//   M = max_i m_i, out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
+// over the pieces of the row's prefix unit and of its own keys' unit, whose places
+// follow from the cost sums that the first launch left in the workspace.  One wave
+// per row, as pa_reduce.hip: lane (r, c) reads dims 4c .. 4c + 3 of every RI-th
+// state, a round of NL loads covers NL * RI of them.
+#include "pa_shared.hpp"
+
+namespace pa {
+
+constexpr int kMergeWaves = 4;
+
+template <int D>
+__global__ __launch_bounds__(64 * kMergeWaves) void shared_merge_kernel(const SharedParams p) {
+  constexpr int LR = D / 4;   // lanes per state
+  constexpr int RI = 64 / LR; // states per load instruction
+  constexpr int NL = 8;       // loads per lane per round
+  const int lane = threadIdx.x & 63;
+  const int r = lane / LR, c = lane % LR;
+  const int64_t f = (int64_t)blockIdx.x * kMergeWaves + (threadIdx.x >> 6);
+  const int64_t row = f / p.H;  // [B, S]
+  if (row >= (int64_t)p.B * p.S) return;
+  const int h = (int)(f - row * p.H);
+  const int b = (int)(row / p.S), s = (int)(row - (int64_t)b * p.S);
+  const int kvh = h / p.G;
+  const int mine = s * p.G + (h - kvh * p.G);  // row among the sequence's
+  const int32_t* cum = p.ws_meta + 2;
+  const int share = p.ws_meta[0], maxctx = p.MB * p.BS;
+  const int ctx = max(p.context_lens[b], 0);
+  const int keys = ctx - p.S + s + 1;  // that the row attends
+  bool bad = p.ws_meta[1] != 0 || ctx > maxctx;
+
+  // The states: n1 of the prefix from row a1 on, n2 of the own keys from a2 on.
+  int n1 = 0, n2 = 0;
+  int64_t a1 = 0, a2 = 0;
+  auto pieces = [&](int entry, int unit, int rows, int tiles, int& first) {
+    const int cost = tile_cost(p, rows);
+    const int begin = cum[entry] + unit * tiles * cost;
+    first = begin / share;
+    return (begin + (tiles - 1) * cost) / share - first + 1;
+  };
+  if (!bad && keys > 0) {
+    const int g = group_of(p.group_starts, p.NG, b);
+    const int P = g < 0 ? 0 : prefix_of(p.prefix_lens[g]);
+    bad = P > maxctx;
+    if (!bad && P > 0) {
+      const int b0 = p.group_starts[g], rows = (p.group_starts[g + 1] - b0) * p.SG;
+      const int at = (b - b0) * p.SG + mine;
+      int first;
+      n1 = pieces(g, kvh * row_blocks(rows) + at / kSharedWide, rows, tiles_of(P), first);
+      a1 = (int64_t)first * kSharedWide + (int64_t)p.HKV * b0 * p.SG + (int64_t)kvh * rows + at;
+    }
+    if (!bad && ctx > P) {
+      int first;
+      n2 = pieces(p.NG + b, kvh * p.own_rb + mine / kSharedWide, p.SG, tiles_of(ctx - own_first(P)), first);
+      const int step = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
+      a2 = (int64_t)p.wgs * kSharedWide + (int64_t)p.HKV * p.B * p.SG + (int64_t)first * step +
+           ((int64_t)b * p.HKV + kvh) * p.SG + mine;
+    }
+  }
+  const int step1 = kSharedWide, step2 = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
+  auto place = [&](int i) { return i < n1 ? a1 + (int64_t)i * step1 : a2 + (int64_t)(i - n1) * step2; };
+  const int all = n1 + n2;
+  float M = -__builtin_inff();
+  for (int i0 = 0; i0 < all; i0 += 64)
+    M = fmaxf(M, i0 + lane < all ? p.ws_m[place(i0 + lane)] : -__builtin_inff());
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
+  float L = 0.0f;
+  for (int i0 = 0; i0 < all; i0 += 64) {
+    float w = 0.0f;
+    if (i0 + lane < all) {
+      const int64_t at = place(i0 + lane);
+      const float m = p.ws_m[at], l = p.ws_l[at];
+      // (A state that saw no key, or a key that cannot be read, has m = -inf: l says which.)
+      w = m == -__builtin_inff() ? 0.0f : fast_exp2(m - M);
+      L += l != l ? l : w * l;
+    }
+    for (int k = 0; k < 64 && i0 + k < all; k += NL * RI) {
+      float4_t x[NL];
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int i = k + j * RI + r;
+        x[j] = i < 64 && i0 + i < all ? *reinterpret_cast<const float4_t*>(p.ws_acc + place(i0 + i) * D + 4 * c)
+                                      : float4_t{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const float wi = __shfl(w, (k + j * RI + r) & 63, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = wi == 0.0f ? acc[e] : fmaf(wi, x[j][e], acc[e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = LR; o < 64; o <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
+  if (r == 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      store_elem(p.out, p.out_dtype, f * D + 4 * c + e,
+                 bad ? __builtin_nanf("") : keys <= 0 ? 0.0f : acc[e] * p.vscale / L);
+  }
+}
+
+hipError_t launch_shared_merge(const SharedParams& p, hipStream_t stream) {
+  const int64_t waves = (int64_t)p.B * p.S * p.H;
+  const dim3 grid((unsigned)((waves + kMergeWaves - 1) / kMergeWaves)), block(64 * kMergeWaves);
+  note_launch("pa::shared_merge_kernel<%d>", p.D);
+  switch (p.D) {
+    case 32: hipLaunchKernelGGL(shared_merge_kernel<32>, grid, block, 0, stream, p); break;
+    case 64: hipLaunchKernelGGL(shared_merge_kernel<64>, grid, block, 0, stream, p); break;
+    case 128: hipLaunchKernelGGL(shared_merge_kernel<128>, grid, block, 0, stream, p); break;
+    case 256: hipLaunchKernelGGL(shared_merge_kernel<256>, grid, block, 0, stream, p); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace pa

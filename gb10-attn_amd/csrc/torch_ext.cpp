@@ -301,6 +301,21 @@ void op_qk_norm_rope_write_kv_out(const at::Tensor& q, const at::Tensor& key, co
                                  interleaved ? 1 : 0, k_scale, v_scale, stream_of(q)));
 }
 
+void op_shared_prefix_out(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt,
+                          const at::Tensor& ctx, const at::Tensor& group_starts, const at::Tensor& prefix_lens,
+                          double scale, double k_scale, double v_scale, const at::Tensor& out) {
+  Args a = q.dim() == 3 ? prep(q, k, v, bt, ctx, 3, "[B, H, D]") : prep(q, k, v, bt, ctx, 4, "[B, S, H, D]");
+  if (reinterpret_cast<uintptr_t>(a.q.data_ptr()) % 16) a.q = a.q.clone();
+  at::Tensor gs = group_starts.to(a.q.device(), at::kInt).contiguous();
+  at::Tensor pl = prefix_lens.to(a.q.device(), at::kInt).contiguous();
+  c10::DeviceGuard guard(a.q.device());
+  pa_tensor_t o = view(out), qq = view(a.q), kk = view(a.k), vv = view(a.v), bb = view(a.bt), cc = view(a.ctx),
+              gg = view(gs), pp = view(pl);
+  Scratch s = scratch_of(a.q, paged_attention_shared_prefix_workspace_size(&qq, &kk, &bb, &gg));
+  check(paged_attention_shared_prefix(&o, &qq, &kk, &vv, &bb, &cc, &gg, &pp, scale, k_scale, v_scale, s.ptr, s.bytes,
+                                      stream_of(a.q)));
+}
+
 void op_copy_pages(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache, const at::Tensor& src,
                    const at::Tensor& dst) {
   one_device(k_cache, {&src, &dst});
@@ -390,6 +405,8 @@ TORCH_LIBRARY(gb10_attn, m) {
   m.def("qk_norm_rope_write_kv_out(Tensor q, Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
         "Tensor slot_mapping, Tensor cos_sin, Tensor positions, Tensor? q_weight, Tensor? k_weight, float eps, "
         "bool interleaved, float k_scale, float v_scale, Tensor(c!) out) -> ()");
+  m.def("shared_prefix_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, "
+        "Tensor group_starts, Tensor prefix_lens, float scale, float k_scale, float v_scale, Tensor(a!) out) -> ()");
   m.def("copy_pages(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor src, Tensor dst) -> ()");
   m.def("fork_sequences(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor(c!) block_tables, Tensor(d!) context_lens, "
         "Tensor(e!) page_refs, Tensor parents, Tensor rows) -> Tensor");
@@ -406,6 +423,7 @@ TORCH_LIBRARY_IMPL(gb10_attn, CUDA, m) {
   m.impl("prefill_out", &op_prefill_out);
   m.impl("write_kv_into", &op_write_kv_into);
   m.impl("qk_norm_rope_write_kv_out", &op_qk_norm_rope_write_kv_out);
+  m.impl("shared_prefix_out", &op_shared_prefix_out);
   m.impl("copy_pages", &op_copy_pages);
   m.impl("fork_sequences", &op_fork_sequences);
   m.impl("free_sequences", &op_free_sequences);

@@ -136,6 +136,19 @@ class _CAbi:
                                                  v_scale, _stream(q.device)))
 
     @staticmethod
+    def shared_prefix_out(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, scale, k_scale,
+                          v_scale, out):
+        args = _prep(q, k_cache, v_cache, block_tables, context_lens, *((3, "[B, H, D]") if q.dim() == 3
+                                                                        else (4, "[B, S, H, D]")))
+        q = args[0] if args[0].data_ptr() % 16 == 0 else args[0].clone()
+        starts, lens = (t.to(q.device, torch.int32).contiguous() for t in (group_starts, prefix_lens))
+        with torch.cuda.device(q.device):
+            need = lib().paged_attention_shared_prefix_workspace_size(*_refs(q, args[1], args[3], starts))
+            ws = _scratch(need, q.device)
+            check(lib().paged_attention_shared_prefix(*_refs(out, q, *args[1:], starts, lens), scale, k_scale, v_scale,
+                                                      ws.data_ptr(), ws.numel(), _stream(q.device)))
+
+    @staticmethod
     def copy_pages(k_cache, v_cache, src, dst):
         with torch.cuda.device(k_cache.device):
             check(lib().pa_copy_pages(*_refs(k_cache, v_cache, src, dst), _stream(k_cache.device)))
@@ -230,6 +243,22 @@ def paged_attention_prefill_varlen(q, k_cache, v_cache, block_tables, context_le
     k_scale / v_scale dequantise a scaled cache (paged_attention_prefill_varlen_scaled)."""
     return _prefill(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, max_q_len, scale, out_dtype, out,
                     k_scale, v_scale, False)
+
+
+def paged_attention_shared_prefix(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, scale, *,
+                                  out_dtype=torch.float32, out=None, k_scale=1.0, v_scale=1.0):
+    """Attention of groups of consecutive sequences that share a prefix, its K/V read once for up to 128
+    query rows of the group (paged_attention_shared_prefix).
+
+    q [B, H, D] (decode) or [B, S, H, D] (S new rows a sequence, causal); group g is sequences
+    group_starts[g] .. group_starts[g + 1] - 1 and shares its first prefix_lens[g] tokens, read through
+    the block table of its first sequence; tokens past them are each sequence's own.  context_lens
+    count the prefix.  fp16/bf16/FP8 caches; where the tables agree the result is paged_attention_v3's."""
+    _on_gpu(q, k_cache, v_cache)
+    o = _out(q, out_dtype, out)
+    _native().shared_prefix_out(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, float(scale),
+                                float(k_scale), float(v_scale), o)
+    return o
 
 
 def workspace_size(q, k_cache, block_tables, num_splits) -> int:

@@ -329,6 +329,41 @@ int pa_write_kv_scaled(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tens
                        const pa_tensor_t* value, const pa_tensor_t* slot_mapping, double k_scale,
                        double v_scale, void* stream);
 
+/* Attention of a batch whose sequences share prefixes: groups of consecutive
+ * sequences attend a common prefix, whose keys and values are read once for a block
+ * of up to 128 of the group's query rows instead of once per sequence.
+ *   q / out [B, H, D] (one new row a sequence), or [B, S, H, D] (S new rows, the
+ *       last S positions of each context, causal, as paged_attention_prefill);
+ *   block_tables, context_lens: as the other entry points take them, the contexts
+ *       with the prefix;
+ *   group_starts int32 [NG + 1], non-decreasing: sequences group_starts[g] ..
+ *       group_starts[g + 1] - 1 form group g (a sequence of no group, or of a group
+ *       without a prefix, is attended alone);
+ *   prefix_lens int32 [NG]: tokens of the group's prefix, need not fill pages.
+ * Token j of a sequence is read through the block table of its group's first
+ * sequence while j < prefix_lens[g], through its own from there on (its own entries
+ * for pages wholly under the prefix are not read).  Where the tables agree the result
+ * is paged_attention_v3_scaled's / paged_attention_prefill_wmma_scaled's.  A context
+ * shorter than the prefix attends that much of it; context_lens[b] <= 0 gives zero
+ * rows; a row that attends an unreadable page, whose context or prefix exceeds MB *
+ * BS tokens, and every row where group_starts decreases or leaves [0, B], is NaN.
+ * fp16, bf16 or FP8 E4M3 caches (k_scale, v_scale as the scaled entry points), q and
+ * out fp32, fp16 or bf16, q 16-byte aligned, B <= 1024, D in {32, 64, 128, 256}.
+ * Probabilities are carried in 16 bits where out is a 16-bit type, as 16-bit hi + lo
+ * pairs where it is fp32 (an infinite V element may then give NaN in its place).
+ * workspace: device memory of paged_attention_shared_prefix_workspace_size(...)
+ * bytes on the current device, 256-byte aligned, of this call alone.  No reference
+ * counterpart (its decode reads each sequence's whole context,
+ * kernels/paged_attn_v3.cu:80-122). */
+int paged_attention_shared_prefix(pa_tensor_t* out, const pa_tensor_t* q, const pa_tensor_t* k_cache,
+                                  const pa_tensor_t* v_cache, const pa_tensor_t* block_tables,
+                                  const pa_tensor_t* context_lens, const pa_tensor_t* group_starts,
+                                  const pa_tensor_t* prefix_lens, double scale, double k_scale, double v_scale,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+size_t paged_attention_shared_prefix_workspace_size(const pa_tensor_t* q, const pa_tensor_t* k_cache,
+                                                    const pa_tensor_t* block_tables,
+                                                    const pa_tensor_t* group_starts);
+
 /* New queries and keys on their way into the paged cache: the RMS norm of each
  * head, the rotation by position and pa_write_kv_scaled's write in one pass.
  *   y = x * rsqrt(mean(x^2) + eps) * weight    over each head's D elements, where

@@ -185,3 +185,66 @@ def test_page_workspaces(pa):
 def test_nothing_to_do(pa):
     a = page_args(pa, N=0)
     assert copy_call(pa, a) == 0 and fork_call(pa, a, ws=None, size=0) == 0 and free_call(pa, a) == 0
+
+
+# ---------------------------------------------------------- shared prefixes --
+
+SHARED = ("out", "q", "k", "v", "bt", "ctx", "starts", "prefix")
+
+
+def shared_args(pa, B=4, S=None, H=8, HKV=2, D=64, NB=20, BS=16, MB=6, NG=2, kv=F16, qd=F16, od=F32):
+    t = lambda *s, d=I32: T(pa, list(s), d)  # noqa: E731
+    rows = (B, H, D) if S is None else (B, S, H, D)
+    return dict(out=t(*rows, d=od), q=t(*rows, d=qd), k=t(NB, BS, HKV, D, d=kv), v=t(NB, BS, HKV, D, d=kv),
+                bt=t(B, MB), ctx=t(B), starts=t(NG + 1), prefix=t(NG))
+
+
+def shared_call(pa, a, scale=0.1, ks=1.0, vs=1.0, ws=FAKE, size=1 << 40):
+    return pa.lib().paged_attention_shared_prefix(*refs(a[n] for n in SHARED), scale, ks, vs, ws, size, None)
+
+
+@pytest.mark.parametrize("sizes,change,code,msg", [
+    ({}, dict(q=([4, 64], F16)), 1, "q must be [B, H, D] or [B, S, H, D]"),
+    ({}, dict(out=([4, 1, 8, 64], F32)), 1, "out must be [B, H, D]"),
+    (dict(S=3), dict(out=([4, 2, 8, 64], F32)), 1, "out must have the shape of q"),
+    (dict(kv=F32), {}, 1, "need an fp16, bf16 or float8_e4m3fn KV cache"),
+    (dict(kv=F64), {}, 1, "need an fp16, bf16 or float8_e4m3fn KV cache"),
+    (dict(qd=FP8), {}, 1, "q must be float32, float16 or bfloat16"),
+    (dict(od=FP8), {}, 1, "out must be float32, float16 or bfloat16"),
+    (dict(H=9), {}, 1, "n_head must be divisible by n_kv_head"),
+    (dict(D=96), {}, 2, "unsupported head_dim 96"),
+    (dict(B=1025), {}, 2, "at most 1024 sequences"),
+    (dict(NG=1025), {}, 2, "at most 1024 sequences"),
+    ({}, dict(starts=([3], I64)), 1, "group_starts must be int32"),
+    ({}, dict(starts=([0], I32), prefix=([0], I32)), 1, "group_starts must have at least one entry"),
+    ({}, dict(prefix=([3], I32)), 1, "prefix_lens must have 2 entries"),
+    ({}, dict(starts=([3], I32, [2])), 1, "group_starts must be contiguous"),
+    ({}, dict(bt=([3, 6], I32)), 1, "block_tables must have B rows"),
+    ({}, dict(ctx=([5], I32)), 1, "context_lens must have B entries"),
+    ({}, dict(q=([4, 8, 64], F16, [1024, 64, 1])), 1, "q must be contiguous"),
+    ({}, dict(q=([4, 8, 64], F16, None, FAKE + 2)), 2, "16-byte aligned q"),
+    ({}, dict(k=([20, 16, 2, 64], F16, [2052, 128, 64, 1])), 2, "multiples of 16 bytes"),
+])
+def test_shared_prefix_refusals(pa, sizes, change, code, msg):
+    a = shared_args(pa, **sizes)
+    for n, s in change.items():
+        a[n] = T(pa, *s)
+    expect(pa, shared_call(pa, a), code, msg)
+
+
+def test_shared_prefix_scalars_and_null(pa):
+    a = shared_args(pa)
+    for bad in (float("nan"), float("inf"), 1e39):
+        expect(pa, shared_call(pa, a, ks=bad), 1, "must be finite")
+        expect(pa, shared_call(pa, a, vs=bad), 1, "must be finite")
+        expect(pa, shared_call(pa, a, scale=bad), 1, "must be finite")
+    expect(pa, shared_call(pa, a, scale=1e30, ks=1e10), 1, "scale * k_scale must be finite")
+    for n in SHARED:
+        rc = shared_call(pa, {**a, n: None})
+        assert rc == 1, (n, rc)
+    assert shared_call(pa, shared_args(pa, B=0), ws=None, size=0) == 0
+    assert shared_call(pa, shared_args(pa, S=0), ws=None, size=0) == 0
+    size = pa.lib().paged_attention_shared_prefix_workspace_size
+    for sizes in (dict(B=1025), dict(NG=1025), dict(H=9), dict(D=512)):
+        b = shared_args(pa, **sizes)
+        assert size(*refs(b[n] for n in ("q", "k", "bt", "starts"))) == C.c_size_t(-1).value
