@@ -1585,10 +1585,10 @@ extern "C" int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, cons
 // per CU, one at D = 256), or has as many as the keys that the tables can hold make
 // shares of.
 static int plan_shared(SharedParams* p) {
-  int cus = 0, rc;
-  if ((rc = device_cu_count(&cus))) return rc;
   if (p->B > kSharedMaxSeqs || p->NG > kSharedMaxSeqs)
     return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups", kSharedMaxSeqs);
+  int cus = 0, rc;
+  if ((rc = device_cu_count(&cus))) return rc;
   const int64_t sg = (int64_t)p->S * p->G, rows = p->B * sg;
   if (rows >= (1LL << 30)) return fail(PA_ERR_UNSUPPORTED, "too many query rows");
   p->SG = (int32_t)sg;
