@@ -1593,14 +1593,16 @@ static int plan_shared(SharedParams* p) {
   if (rows >= (1LL << 30)) return fail(PA_ERR_UNSUPPORTED, "too many query rows");
   p->SG = (int32_t)sg;
   p->own_rb = (int32_t)((sg + kSharedWide - 1) / kSharedWide);
-  p->cost_thin = 1;
-  p->cost_wide = 1;
-  p->min_share = 4;
-  const int64_t tiles = ((int64_t)p->MB * p->BS + kSharedTile - 1) / kSharedTile + 1;
-  const int64_t units = p->HKV * (rows / kSharedWide + p->NG + (int64_t)p->B * p->own_rb);
-  const int64_t most = units * tiles * std::max(p->cost_thin, p->cost_wide);
-  if (units >= (1LL << 31) || most >= (1LL << 31)) return fail(PA_ERR_UNSUPPORTED, "too many keys and query rows for one call");
-  p->wgs = (int32_t)std::min<int64_t>((p->D <= 128 ? 2 : 1) * (int64_t)cus, std::max<int64_t>(1, (most + p->min_share - 1) / p->min_share));
+  p->thin = sg <= kSharedThin;
+  p->page16 = p->BS % 16 == 0;
+  // The longest line: every unit over all the keys that a table row holds.
+  const int64_t keys = (int64_t)p->MB * p->BS + 16;
+  const int64_t wide = kSharedWideStart + kSharedWideCost * ((keys + kSharedWideTile - 1) / kSharedWideTile);
+  const int64_t thin = kSharedThinStart + kSharedThinCost * ((keys + kSharedThinTile - 1) / kSharedThinTile);
+  const int64_t units = p->HKV * (rows / kSharedWide + p->NG), own = (int64_t)p->HKV * p->B * p->own_rb;
+  const double most = (double)units * (double)wide + (double)own * (double)(p->thin ? thin : wide);
+  if (most >= (double)(1LL << 31) - 1e6) return fail(PA_ERR_UNSUPPORTED, "too many keys and query rows for one call");
+  p->wgs = (int32_t)std::min<int64_t>((p->D <= 128 ? 2 : 1) * (int64_t)cus, (int64_t)most / kSharedMinShare + 1);
   p->sg_div = make_fastdiv((uint32_t)std::max(1, p->SG));
   p->g_div = make_fastdiv((uint32_t)std::max(1, p->G));
   return PA_OK;
@@ -1608,8 +1610,7 @@ static int plan_shared(SharedParams* p) {
 
 static size_t shared_meta_bytes(const SharedParams& p) { return (4 * (size_t)(3 + p.NG + p.B) + 255) & ~(size_t)255; }
 static size_t shared_rows(const SharedParams& p) {
-  const size_t own = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
-  return (size_t)p.wgs * (kSharedWide + own) + 2 * (size_t)p.HKV * p.B * p.SG;
+  return (size_t)p.wgs * (kSharedWide + (p.thin ? 4 * kSharedThin : kSharedWide)) + 2 * (size_t)p.HKV * p.B * p.SG;
 }
 static size_t shared_bytes(const SharedParams& p) { return shared_meta_bytes(p) + shared_rows(p) * (p.D + 2) * 4; }
 
@@ -1695,7 +1696,11 @@ extern "C" int paged_attention_shared_prefix(pa_tensor_t* out, const pa_tensor_t
   p.NG = (int32_t)(group_starts->shape[0] - 1);
   p.q_dtype = d.q_dtype; p.out_dtype = d.out_dtype;
   p.bs_div = d.bs_div;
-  p.qscale = (float)(scale * k_scale * 1.4426950408889634);
+  const float qs = (float)(scale * k_scale * 1.4426950408889634);
+  p.qscale = qs == 0.0f ? 1.0f : std::max(std::fabs(qs), 0x1p-126f);
+  p.q_sign = qs == 0.0f ? 0.0f : qs < 0.0f ? -1.0f : 1.0f;
+  p.q_and = qs == 0.0f ? 0u : 0xffffffffu;
+  p.q_xor = qs < 0.0f ? 0x80008000u : 0u;
   p.vscale = (float)v_scale;
   if ((rc = plan_shared(&p))) return rc;
   if ((rc = check_scratch(shared_bytes(p), workspace, workspace_bytes))) return rc;

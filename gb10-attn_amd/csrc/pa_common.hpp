@@ -316,21 +316,30 @@ struct SharedParams {
   int32_t B, S, H, HKV, G, D, BS, MB, NG;
   int32_t SG;      // S * G: query rows of a sequence under one KV head
   int32_t own_rb;  // row blocks of a sequence's own keys
+  int32_t thin;    // 1: a sequence's rows fit one thin unit
+  int32_t page16;  // 1: sixteen rows from a multiple of 16 on lie in one page
   int32_t q_dtype, out_dtype;
-  int32_t wgs;               // work-groups of the grid
-  int32_t cost_thin, cost_wide;  // of a tile of keys, in the units that are shared out
-  int32_t min_share;         // fewest units of a work-group
+  int32_t wgs;     // work-groups of the grid
   FastDiv bs_div, sg_div, g_div;
-  float qscale, vscale;
+  float qscale;           // |scale| * k_scale * log2 e, or 1 where that is 0
+  float q_sign;           // its sign, or 0, applied to q
+  uint32_t q_and, q_xor;  // the same on packed 16-bit q: bits & q_and ^ q_xor
+  float vscale;
   // Workspace: share, fault and the cost sums; the pieces' softmax states.
   int32_t* ws_meta;  // [2 + NG + 1 + B + 1]
   float* ws_acc;     // [rows][D]
   float* ws_m;       // [rows] log2 units
   float* ws_l;       // [rows]
 };
-constexpr int kSharedWide = 128;  // query rows of a wide unit
-constexpr int kSharedThin = 16;   // ... of a thin one
-constexpr int kSharedTile = 64;   // keys of a tile
+constexpr int kSharedWide = 128;      // query rows of a wide unit
+constexpr int kSharedThin = 16;       // ... of a thin one
+constexpr int kSharedWideTile = 64;   // keys of a tile of either
+constexpr int kSharedThinTile = 32;
+// Cost of a tile and of a unit's start, in the parts that are shared out (about
+// 0.3 us of a work-group; a thin tile is a wave's, four at a time).
+constexpr int kSharedWideCost = 4, kSharedWideStart = 8;
+constexpr int kSharedThinCost = 3, kSharedThinStart = 2;
+constexpr int kSharedMinShare = 4 * kSharedThinCost;  // a wave's share holds the start of a tile
 constexpr int kSharedMaxSeqs = 1024;
 
 constexpr int kDecodeWaves = 4;

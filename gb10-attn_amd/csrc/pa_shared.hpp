@@ -9,21 +9,22 @@
 //
 // Work.  A unit is a block of query rows against one run of keys under one KV
 // head: the rows of a whole group against its prefix, the rows of a sequence
-// against its own keys.  The units' tiles of 64 keys lie end to end on a line, in
-// units of cost, and every work-group takes an equal stretch of it, cutting units
-// where the stretch ends: no work-group waits for a longer one whatever the
-// lengths, and compute-bound prefixes run beside memory-bound tails.  A stretch's
-// piece of a unit is one state per row.  A piece's rows have a place of their own
-// in the workspace without any table: work-group w's stretch and unit u's first row
-// only grow along the line, so w * 128 + row is unique.
+// against its own keys.  The units' key tiles lie end to end on a line, measured in
+// cost, and every worker takes an equal stretch of it, cutting units where the
+// stretch ends: nobody waits for a longer one whatever the lengths, and
+// compute-bound prefixes run beside memory-bound tails.  A worker's piece of a unit
+// leaves one state per row.  Its place in the workspace needs no table: worker w's
+// stretch and unit u's first row only grow along the line, so w * 128 + row (16 for
+// thin units) is unique.
 //
 // Two bodies, on v_mfma_f32_{32x32x16,16x16x32}:
-//  * wide, up to 128 rows: a wave owns 32 rows, the tile's K and V go through LDS
-//    once for all four (two tiles in flight).  One read of the prefix serves 128
-//    rows.
-//  * thin, up to 16 rows: memory-bound.  The waves take 32-key tiles in turn, K
-//    straight into the operand registers, V through the wave's own LDS; their
-//    states are joined in LDS at the end of the piece.
+//  * wide, up to 128 rows (every prefix, and own keys under more than 16 rows): a
+//    work-group is the worker.  A wave owns 32 rows; a tile's K and V go through
+//    LDS once for all four, the next tile's loads in flight.  One read of the
+//    prefix serves 128 rows.
+//  * thin, up to 16 rows: memory-bound.  A wave is the worker, each with its own
+//    units and no barrier, since tails are short and a unit's chain of loads long.
+//    K goes straight into the operand registers, V through the wave's own LDS.
 // Both compute S^T = K Q^T, whose accumulator layout is the operand layout of
 // O^T += V^T P^T: the probabilities stay in registers.
 //
@@ -98,7 +99,9 @@ __device__ inline float v_elem(const char* vbase, uint64_t off, int d) {
 // ------------------------------------------------------------------- plan --
 
 struct ShPlan {
-  int total, share;
+  int total;  // end of the line
+  int own;    // where the sequences' own keys begin
+  int share;  // a work-group's stretch, a multiple of 4
 };
 
 // A sequence's group, or -1.  starts: [NG + 1], non-decreasing.
@@ -112,25 +115,30 @@ __device__ inline int group_of(const int32_t* starts, int NG, int b) {
   return lo;
 }
 
-__device__ inline int tiles_of(int n) { return (n + kSharedTile - 1) / kSharedTile; }
 __device__ inline int row_blocks(int rows) { return (rows + kSharedWide - 1) / kSharedWide; }
-__device__ inline int tile_cost(const SharedParams& p, int rows) {
-  return rows <= kSharedThin ? p.cost_thin : p.cost_wide;
+__device__ inline int wide_tiles(int n) { return (n + kSharedWideTile - 1) / kSharedWideTile; }
+__device__ inline int own_tiles(const SharedParams& p, int n) {
+  return p.thin ? (n + kSharedThinTile - 1) / kSharedThinTile : wide_tiles(n);
 }
-// First key of the tiles of a sequence's own keys: pages of 16 and more tokens
-// then hold 16 rows of a tile each.
+__device__ inline int wide_cost(int tiles) { return kSharedWideStart + tiles * kSharedWideCost; }
+__device__ inline int own_cost(const SharedParams& p, int tiles) {
+  return p.thin ? kSharedThinStart + tiles * kSharedThinCost : wide_cost(tiles);
+}
+// First key of the tiles of a sequence's own keys: sixteen rows of a tile then lie
+// in one page where pages hold a multiple of 16.
 __device__ inline int own_first(int prefix) { return prefix & ~15; }
 // Prefix of a group as attended: none where it is negative.
 __device__ inline int prefix_of(int n) { return n > 0 ? n : 0; }
 
-// Sums of the units' costs, prefixes first, in s_cum [NG + 1 + B] (s_cum[i]: before
-// entry i), and whether the group starts are unusable.  s_tmp: scratch of 2 NG + 1
-// + 8 words.  Every thread of the work-group.
-__device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_t* s_tmp, int& fault) {
+// Where the units lie on the line: s_cum[i] is the cost before entry i (groups, then
+// sequences), s_pre[b] the prefix of sequence b.  s_tmp: scratch of 2 NG + 1 + 8
+// words.  Every thread of the work-group; fault: the group starts are unusable.
+__device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_t* s_pre, int32_t* s_tmp, int& fault) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* s_start = s_tmp + 8;
   int32_t* s_len = s_start + p.NG + 1;
   const int maxctx = p.MB * p.BS;
+  int ctx = tid < p.B ? p.context_lens[tid] : 0;  // (in flight beside the groups)
   int bad = 0;
   for (int g = tid; g <= p.NG; g += kShThreads) {
     const int a = p.group_starts[g];
@@ -139,21 +147,9 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_
     if (g < p.NG) s_len[g] = prefix_of(p.prefix_lens[g]);
   }
   fault = __syncthreads_or(bad);
-  if (fault) return {0, 1};
+  if (fault) return {0, 0, 4};
   int carry = 0;
-  const int n = p.NG + p.B;
-  for (int i0 = 0; i0 < n; i0 += kShThreads) {
-    const int i = i0 + tid;
-    int c = 0;
-    if (i < p.NG) {
-      const int rows = (s_start[i + 1] - s_start[i]) * p.SG, len = s_len[i];
-      if (len <= maxctx) c = p.HKV * row_blocks(rows) * tiles_of(len) * tile_cost(p, rows);
-    } else if (i < n) {
-      const int b = i - p.NG;
-      const int g = group_of(s_start, p.NG, b);
-      const int P = g < 0 ? 0 : s_len[g], ctx = p.context_lens[b];
-      if (ctx > P && ctx <= maxctx) c = p.HKV * p.own_rb * tiles_of(ctx - own_first(P)) * tile_cost(p, p.SG);
-    }
+  auto scan = [&](int i, int n, int c, int32_t* cum) {
     int x = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -168,16 +164,59 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_
       before += w < wave ? s_tmp[w] : 0;
       carry += s_tmp[w];
     }
-    if (i < n) s_cum[i] = before + x - c;
+    if (i < n) cum[i] = before + x - c;
     __syncthreads();
+  };
+  for (int i0 = 0; i0 < p.NG; i0 += kShThreads) {
+    const int g = i0 + tid;
+    int c = 0;
+    if (g < p.NG && s_len[g] > 0 && s_len[g] <= maxctx)
+      c = p.HKV * row_blocks((s_start[g + 1] - s_start[g]) * p.SG) * wide_cost(wide_tiles(s_len[g]));
+    scan(g, p.NG, c, s_cum);
   }
-  if (tid == 0) s_cum[n] = carry;
+  const int own = carry;
+  for (int i0 = 0; i0 < p.B; i0 += kShThreads) {
+    const int b = i0 + tid;
+    int c = 0;
+    if (b < p.B) {
+      if (i0 > 0) ctx = p.context_lens[b];
+      const int g = group_of(s_start, p.NG, b);
+      const int P = g < 0 ? 0 : s_len[g];
+      s_pre[b] = P;
+      if (ctx > P && ctx <= maxctx) c = p.HKV * p.own_rb * own_cost(p, own_tiles(p, ctx - own_first(P)));
+    }
+    scan(b, p.B, c, s_cum + p.NG);
+  }
+  if (tid == 0) s_cum[p.NG + p.B] = carry;
   __syncthreads();
-  return {carry, max(p.min_share, (carry + p.wgs - 1) / p.wgs)};
+  const int even = (carry + p.wgs - 1) / p.wgs;
+  return {carry, own, max(kSharedMinShare, (even + 3) & ~3)};
 }
 
-// One piece: rows [row0, row0 + rows) of the block's numbering against the keys of
-// tiles [k0, k1) of a unit.
+// Which states a unit left: workers first .. last, for tiles of `cost` behind `start`
+// of a unit that begins at `begin`.
+__device__ inline void unit_workers(int begin, int start, int cost, int tiles, int share, int& first, int& count) {
+  first = (begin + start) / share;
+  count = (begin + start + (tiles - 1) * cost) / share - first + 1;
+}
+
+// Rows of the workspace: the prefixes' states, then the own keys'.
+__host__ __device__ inline int64_t prefix_slots(const SharedParams& p) {
+  return (int64_t)p.wgs * kSharedWide + (int64_t)p.HKV * p.B * p.SG;
+}
+__host__ __device__ inline int64_t own_slots(const SharedParams& p) {
+  return (int64_t)p.wgs * (p.thin ? kShWaves * kSharedThin : kSharedWide) + (int64_t)p.HKV * p.B * p.SG;
+}
+__device__ inline int64_t prefix_slot(const SharedParams& p, int worker, int b0, int rows, int kvh, int row) {
+  return (int64_t)worker * kSharedWide + (int64_t)p.HKV * b0 * p.SG + (int64_t)kvh * rows + row;
+}
+__device__ inline int64_t own_slot(const SharedParams& p, int worker, int b, int kvh, int row) {
+  return prefix_slots(p) + (int64_t)worker * (p.thin ? kSharedThin : kSharedWide) +
+         ((int64_t)b * p.HKV + kvh) * p.SG + row;
+}
+
+// One piece: rows [row0, row0 + rows) of the unit's numbering against the keys of
+// tiles [k0, k1).
 struct ShPiece {
   int kvh;
   int b0;       // sequence of row 0 of the unit's numbering
@@ -206,30 +245,32 @@ __device__ inline void row_of(const SharedParams& p, const ShPiece& u, int r, bo
   lim = live ? n : 0x7fffffff;
 }
 
-// q row at dims d0 + 32 st .. of 8 (NS steps of `stride` dims) as hi (+ lo) words of
-// the tiles' type.  fp16 hi + lo rows are scaled by the power of two that puts the
-// row's largest element in [2^14, 2^15), and their scores by the inverse, returned
-// in `back` (other: a lane that holds other dims of the row, xor'ed in steps).
+// q row at dims d0 + kStep ks .. of 8 as hi (+ lo) words of the tiles' type, with the
+// scale's sign.  fp16 hi + lo rows are scaled by the power of two that puts the row's
+// largest element in [2^14, 2^15), and their scores by the inverse, returned in
+// `back` (lanes kFrom, 2 kFrom, .. apart hold the row's other dims).
 template <bool kBf, bool kSplit, int NS, int kStep, int kFrom>
 __device__ inline void load_q(const SharedParams& p, bool live, int64_t qrow, int d0, u32x4_t (&hi)[NS],
                               u32x4_t (&lo)[kSplit ? NS : 1], float& back) {
   back = 1.0f;
   if constexpr (!kSplit) {
+    const uint32_t a = live ? p.q_and : 0u, x = live ? p.q_xor : 0u;
+#pragma unroll
+    for (int ks = 0; ks < NS; ++ks) hi[ks] = load16(p.q, (qrow * p.D + d0 + kStep * ks) * 2);
 #pragma unroll
     for (int ks = 0; ks < NS; ++ks) {
-      hi[ks] = load16(p.q, (qrow * p.D + d0 + kStep * ks) * 2);
-      if (!live) hi[ks] = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) hi[ks][j] = (hi[ks][j] & a) ^ x;
     }
     return;
   }
   float x[NS][8];
+  const float sign = live ? p.q_sign : 0.0f;
 #pragma unroll
   for (int ks = 0; ks < NS; ++ks) {
     load8f(p.q, p.q_dtype, qrow * p.D + d0 + kStep * ks, x[ks]);
-    if (!live) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[ks][e] = 0.0f;
-    }
+    for (int e = 0; e < 8; ++e) x[ks][e] = sign == 0.0f ? 0.0f : x[ks][e] * sign;
   }
   if constexpr (kSplit && !kBf) {
     float mx = 0.0f;
@@ -266,9 +307,9 @@ __device__ inline void load_q(const SharedParams& p, bool live, int64_t qrow, in
   }
 }
 
-// Byte offsets of one key row's K and V under the piece's head, and what is wrong
-// with it: a row past the unit, or on a page outside the cache, is read at row 0 of
-// block 0 (in bounds, NB >= 1) and not used.
+// Byte offsets of one key row's K and V under the piece's head.  A row past the
+// unit, or on a page outside the cache, is read at row 0 of block 0 (in bounds, NB >=
+// 1) and not used.
 struct ShRow {
   uint64_t k, v;
   bool use, bad;
@@ -288,26 +329,24 @@ __device__ inline uint64_t shfl64(uint64_t x, int lane) {
   return ((uint64_t)b << 32) | a;
 }
 
-// ------------------------------------------------------------------- wide --
+// ------------------------------------------------------------------- tiles --
 
 template <int D>
 struct ShShape {
-  static constexpr int KB = D <= 128 ? 64 : 32;    // keys per LDS tile of the wide body
+  static constexpr int KB = D <= 128 ? 64 : 32;  // keys per LDS tile of the wide body
   static constexpr int MT = KB / 32;
   static constexpr int KS = D / 16;
   static constexpr int DT = D / 32;
   static constexpr int NCH = D / 8;
-  static constexpr int TPD = 64 / NCH;             // rows per 1 KB load
-  static constexpr int RPW = KB / kShWaves;        // rows a wave loads
-  static constexpr int NP = RPW / TPD;             // loads per wave and tile
-  static constexpr int TILE = KB * D;              // 16-bit elements
-  static constexpr int KT = 32;                    // keys per wave tile of the thin body
-  static constexpr int NDMA = KT / TPD;
-  static constexpr int LDS_WIDE = 4 * TILE * 2;    // K and V, two tiles
-  static constexpr int LDS_THIN = kShWaves * KT * D * 2 > kShWaves * 16 * D * 4 ? kShWaves * KT * D * 2
-                                                                               : kShWaves * 16 * D * 4;
-  static constexpr int LDS_BODY = LDS_WIDE > LDS_THIN ? LDS_WIDE : LDS_THIN;
+  static constexpr int TPD = 64 / NCH;       // rows per 1 KB load
+  static constexpr int RPW = KB / kShWaves;  // rows a wave loads
+  static constexpr int NP = RPW / TPD;       // loads per wave and tile
+  static constexpr int TILE = KB * D;        // 16-bit elements
+  static constexpr int NDMA = kSharedThinTile / TPD;  // V loads of a thin tile
+  static constexpr int LDS_WIDE = 4 * TILE * 2;       // K and V, two tiles
+  static constexpr int LDS_THIN = kShWaves * kSharedThinTile * D * 2;
   static constexpr int LDS_PLAN = (8 + 2 * kSharedMaxSeqs + 1) * 4;
+  static constexpr int LDS_BODY = LDS_WIDE > LDS_THIN ? LDS_WIDE : LDS_THIN;
   static constexpr int LDS = LDS_BODY > LDS_PLAN ? LDS_BODY : LDS_PLAN;
   static_assert(NP >= 1 && RPW % TPD == 0, "tile shape");
 };
@@ -316,23 +355,24 @@ struct ShFlags {
   unsigned long long bad[3];  // per tile, three in turn: keys on pages outside the cache
   int odd;                    // something was taken out of V (restore_odd)
   int lim[kSharedWide];       // end of the keys that each row attends
+  int shortest[kShWaves];
 };
 
 // Adds to the piece's states what sanitize() took out of V: the elements that are not
 // finite, in tiles of KT keys that some row does not see whole (the shortest row ends
-// at `least`), for the rows that see their keys.
+// at `least`), for the rows that see their keys.  `tid` of `threads` threads.
 template <typename KV>
-__device__ __forceinline__ void restore_odd(const SharedParams& p, const ShPiece& u, const int* lim, int least, int KT) {
-  __syncthreads();  // the states and limits are written
+__device__ __forceinline__ void restore_odd(const SharedParams& p, const ShPiece& u, const int* lim, int least, int KT,
+                                            int step, int tid, int threads) {
   const char* vbase = static_cast<const char*>(p.v) + (int64_t)u.kvh * p.v_sh * KV::kBytes;
-  const int n0 = u.first + u.k0 * kSharedTile, n1 = min(u.first + u.k1 * kSharedTile, u.end);
+  const int n0 = u.first + u.k0 * step, n1 = min(u.first + u.k1 * step, u.end);
   for (int key = max(n0, u.lo); key < n1; ++key) {
     const int t0 = n0 + (key - n0) / KT * KT;
     if (t0 >= u.lo && t0 + KT <= least) continue;
     const int pg = (int)fastdiv((uint32_t)key, p.bs_div);
     const ShRow row = key_row(p, u.table[pg], key - pg * p.BS, true, KV::kBytes);
     if (row.bad) continue;
-    for (int d = threadIdx.x; d < p.D; d += kShThreads) {
+    for (int d = tid; d < p.D; d += threads) {
       const float x = v_elem<KV>(vbase, row.v, d);
       if (__builtin_isfinite(x)) continue;
       for (int r = 0; r < u.rows; ++r)
@@ -341,8 +381,26 @@ __device__ __forceinline__ void restore_odd(const SharedParams& p, const ShPiece
   }
 }
 
+// The softmax step over N raw scores of a lane's row (kOther: the lanes that hold its
+// other keys): raises the running maximum m (log2 units) where it is passed by more
+// than 2^8 and says by what the sums shrink.
+template <int kOther>
+__device__ inline float raise_max(float mx, float qscale, float& m) {
+#pragma unroll
+  for (int o = kOther; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  mx *= qscale;
+  if (__builtin_amdgcn_ballot_w64(mx > m + kLazyRescale) == 0) return 1.0f;
+  asm volatile("");
+  const float mn = fmaxf(m, mx);
+  const float corr = mn == -__builtin_inff() ? 1.0f : fast_exp2(m - mn);
+  m = mn;
+  return corr;
+}
+
+// ------------------------------------------------------------------- wide --
+
 template <typename KV, bool kBf, int D, bool kSplitQ, bool kSplitP>
-__device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece& u, char* lds, ShFlags* fl, int* s_min) {
+__device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece& u, char* lds, ShFlags* fl) {
   using Sh = ShShape<D>;
   using Tl = ShTile<KV, kBf>;
   constexpr int KB = Sh::KB, MT = Sh::MT, KS = Sh::KS, DT = Sh::DT, NCH = Sh::NCH, TPD = Sh::TPD, RPW = Sh::RPW,
@@ -354,6 +412,29 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hh = lane >> 5;
 
+  const char* kbase = static_cast<const char*>(p.k) + (int64_t)u.kvh * p.k_sh * EB;
+  const char* vbase = static_cast<const char*>(p.v) + (int64_t)u.kvh * p.v_sh * EB;
+  const int n0 = u.first + u.k0 * kSharedWideTile;  // first key of the piece
+  const int n1 = min(u.first + u.k1 * kSharedWideTile, u.end);
+  const int ntiles = (n1 - n0 + KB - 1) / KB;
+
+  // This wave loads rows [RPW wave, RPW wave + RPW) of a tile.  Where they lie in one
+  // page its block id is a scalar and a lane's part of the addresses a constant;
+  // else lane r holds the page of row r % RPW.
+  const int myrow = wave * RPW + (p.page16 ? 0 : lane % RPW);
+  auto page_at = [&](int tile) {
+    const int pg = (int)fastdiv((uint32_t)min(n0 + tile * KB + myrow, n1 - 1), p.bs_div);
+    return u.table[pg];
+  };
+  int32_t blk = page_at(0);
+  uint32_t klane[NP], vlane[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int r = i * TPD + lane / NCH, row = wave * RPW + r;
+    klane[i] = (uint32_t)r * (uint32_t)(p.k_st * EB) + kpos<D>(row, lane % NCH) * 8 * EB;
+    vlane[i] = (uint32_t)r * (uint32_t)(p.v_st * EB) + vpos<D>(row, lane % NCH) * 8 * EB;
+  }
+
   bool live;
   int64_t qrow;
   int lim;
@@ -362,79 +443,92 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   u32x4_t qf[KS], ql[kSplitQ ? KS : 1];
   float back;
   load_q<kBf, kSplitQ, KS, 16, 32>(p, live, qrow, hh * 8, qf, ql, back);
-  const float qscale = p.qscale * back;
+  const float qscale = kSplitQ && !kBf ? fmaxf(p.qscale * back, 0x1p-126f) : p.qscale;
 
   // The shortest row of this wave and of the block.
   int wmin = lim;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) wmin = min(wmin, __shfl_xor(wmin, o, 64));
   wmin = __builtin_amdgcn_readfirstlane(wmin);
-  if (lane == 0) s_min[wave] = wmin;
+  if (lane == 0) fl->shortest[wave] = wmin;
   if (hh == 0) fl->lim[wave * 32 + lane] = lim;
   if (threadIdx.x < 3) fl->bad[threadIdx.x] = 0;
   if (threadIdx.x == 0) fl->odd = 0;
   __syncthreads();
-  const int bmin = min(min(s_min[0], s_min[1]), min(s_min[2], s_min[3]));
+  const int bmin = __builtin_amdgcn_readfirstlane(
+      min(min(fl->shortest[0], fl->shortest[1]), min(fl->shortest[2], fl->shortest[3])));
 
-  const char* kbase = static_cast<const char*>(p.k) + (int64_t)u.kvh * p.k_sh * EB;
-  const char* vbase = static_cast<const char*>(p.v) + (int64_t)u.kvh * p.v_sh * EB;
-  const int n0 = u.first + u.k0 * kSharedTile;  // first key of the piece
-  const int n1 = min(u.first + u.k1 * kSharedTile, u.end);
-  const int ntiles = (n1 - n0 + KB - 1) / KB;
-
-  // This wave loads rows [RPW wave, RPW wave + RPW) of a tile; lane r holds row
-  // r % RPW's page.
-  const int myrow = wave * RPW + lane % RPW;
-  auto page_at = [&](int tile, int& off) {
-    const int key = n0 + tile * KB + myrow;
-    const int kk = min(key, n1 - 1);
-    const int pg = (int)fastdiv((uint32_t)kk, p.bs_div);
-    off = kk - pg * p.BS;
-    return u.table[pg];
-  };
-  uint32_t use = 0;                      // bit i: this lane's row of load i is used
+  uint32_t dead = 0;  // bit i: this lane's row of load i is not used
   typename Tl::Raw kr[Tl::kF8 ? NP : 1], vr[Tl::kF8 ? NP : 1];
-  ShRow mine;
-  auto issue = [&](int tile, int32_t blk, int off) {
-    mine = key_row(p, blk, off, n0 + tile * KB + myrow < n1, EB);
-    if (mine.bad && lane < RPW) atomicOr(&fl->bad[tile % 3], 1ull << myrow);
-    use = 0;
-    uint16_t* dK = sK + (tile & 1) * Sh::TILE + wave * RPW * D;
-    uint16_t* dV = sV + (tile & 1) * Sh::TILE + wave * RPW * D;
+  auto issue = [&](int tile, int slot3, uint16_t* dK, uint16_t* dV) {
+    const int key = n0 + tile * KB + wave * RPW;  // first of this wave's rows
+    dead = 0;
+    if (p.page16) {
+      const int32_t id = __builtin_amdgcn_readfirstlane(blk);
+      const bool ok = (uint64_t)(int64_t)id < (uint64_t)p.num_blocks;
+      const bool use = ok && key < n1;
+      if (!ok && key < n1 && lane == 0)
+        atomicOr(&fl->bad[slot3], ((1ull << min(RPW, n1 - key)) - 1) << (wave * RPW));
+      const uint32_t ub = use ? (uint32_t)id : 0u;
+      const uint32_t uo = use ? (uint32_t)key - fastdiv((uint32_t)key, p.bs_div) * (uint32_t)p.BS : 0u;
+      const char* ka = kbase + ((uint64_t)ub * (uint32_t)(p.k_sb * EB) + uo * (uint32_t)(p.k_st * EB));
+      const char* va = vbase + ((uint64_t)ub * (uint32_t)(p.v_sb * EB) + uo * (uint32_t)(p.v_st * EB));
+      // (A page holds RPW rows and more, so those past the unit's end exist too.)
+      if (!use || key + RPW > n1) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int r = i * TPD + lane / NCH, row = wave * RPW + r;
-      const uint64_t ko = shfl64(mine.k, r), vo = shfl64(mine.v, r);
-      use |= (uint32_t)__shfl((int)mine.use, r, 64) << i;
-      const char* ka = kbase + ko + kpos<D>(row, lane % NCH) * 8 * EB;
-      const char* va = vbase + vo + vpos<D>(row, lane % NCH) * 8 * EB;
-      if constexpr (Tl::kF8) {
-        kr[i] = *reinterpret_cast<const typename Tl::Raw*>(ka);
-        vr[i] = *reinterpret_cast<const typename Tl::Raw*>(va);
-      } else {
-        lds_dma16_async(ka, (lds_void_t*)(dK + i * 512));
-        lds_dma16_async(va, (lds_void_t*)(dV + i * 512));
+        for (int i = 0; i < NP; ++i) dead |= (uint32_t)(!use || key + i * TPD + lane / NCH >= n1) << i;
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if constexpr (Tl::kF8) {
+          kr[i] = *reinterpret_cast<const typename Tl::Raw*>(ka + klane[i]);
+          vr[i] = *reinterpret_cast<const typename Tl::Raw*>(va + vlane[i]);
+        } else {
+          lds_dma16_async(ka + klane[i], (lds_void_t*)(dK + wave * RPW * D + i * 512));
+          lds_dma16_async(va + vlane[i], (lds_void_t*)(dV + wave * RPW * D + i * 512));
+        }
+      }
+    } else {
+      const int mine = n0 + tile * KB + myrow;
+      const int kk = min(mine, n1 - 1);
+      const ShRow row = key_row(p, blk, kk - (int)fastdiv((uint32_t)kk, p.bs_div) * p.BS, mine < n1, EB);
+      if (row.bad && lane < RPW) atomicOr(&fl->bad[slot3], 1ull << myrow);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int r = i * TPD + lane / NCH;
+        dead |= (uint32_t)(__shfl((int)row.use, r, 64) == 0) << i;
+        const char* ka = kbase + shfl64(row.k, r) + kpos<D>(wave * RPW + r, lane % NCH) * 8 * EB;
+        const char* va = vbase + shfl64(row.v, r) + vpos<D>(wave * RPW + r, lane % NCH) * 8 * EB;
+        if constexpr (Tl::kF8) {
+          kr[i] = *reinterpret_cast<const typename Tl::Raw*>(ka);
+          vr[i] = *reinterpret_cast<const typename Tl::Raw*>(va);
+        } else {
+          lds_dma16_async(ka, (lds_void_t*)(dK + wave * RPW * D + i * 512));
+          lds_dma16_async(va, (lds_void_t*)(dV + wave * RPW * D + i * 512));
+        }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
   // The tile's loads have landed: widen FP8 codes, zero the V rows that are not
   // used, take out what is not finite where some row does not see the whole tile.
-  auto finish = [&](int tile) {
+  auto finish = [&](int tile, uint16_t* dK, uint16_t* dV) {
     const int t0 = n0 + tile * KB;
     const bool masked = t0 < u.lo || t0 + KB > bmin;
-    uint16_t* dK = sK + (tile & 1) * Sh::TILE + wave * RPW * D + lane * 8;
-    uint16_t* dV = sV + (tile & 1) * Sh::TILE + wave * RPW * D + lane * 8;
+    dK += wave * RPW * D + lane * 8;
+    dV += wave * RPW * D + lane * 8;
+    if constexpr (Tl::kF8) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      u32x4_t x;
-      if constexpr (Tl::kF8) {
+      for (int i = 0; i < NP; ++i) {
         *reinterpret_cast<u32x4_t*>(dK + i * 512) = Tl::widen(kr[i]);
-        x = Tl::widen(vr[i]);
+        *reinterpret_cast<u32x4_t*>(dV + i * 512) = Tl::widen(vr[i]);
       }
-      const bool dead = !((use >> i) & 1u);
-      if (Tl::kF8 || dead || masked) {
-        if constexpr (!Tl::kF8) x = *reinterpret_cast<const u32x4_t*>(dV + i * 512);
-        if (dead) {
+    }
+    if (masked || __builtin_amdgcn_ballot_w64(dead != 0) != 0) {
+#pragma unroll 1
+      for (int i = 0; i < NP; ++i) {
+        u32x4_t x = *reinterpret_cast<const u32x4_t*>(dV + i * 512);
+        if ((dead >> i) & 1u) {
           x = u32x4_t{0u, 0u, 0u, 0u};
         } else if (masked && sanitize<kBf>(x)) {
           fl->odd = 1;
@@ -452,28 +546,66 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   }
   float m = -__builtin_inff(), l = 0.0f;
 
-  auto compute = [&](int tile) {
-    const uint16_t* cK = sK + (tile & 1) * Sh::TILE;
-    const uint16_t* cV = sV + (tile & 1) * Sh::TILE;
+  // LDS addresses of the operands: K chunk of k-step ks (m-tiles 32 rows apart), V of
+  // dim tile dt (16-key steps 16 rows apart, the operand's second half 8).
+  int kat[KS], vat[DT];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) kat[ks] = swk<D>(lane & 31, 2 * ks + hh);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int c = dt * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    vat[dt] = swv<D>(4 * hh + ((lane & 15) >> 2), c >> 3) + (c & 7);
+  }
+  static_assert(((8 >> PfShape<D>::VSH) & PfShape<D>::VSW) == 0 && ((16 >> PfShape<D>::VSH) & PfShape<D>::VSW) == 0 &&
+                    ((32 >> PfShape<D>::KSH) & PfShape<D>::KSW) == 0,
+                "the swizzles repeat every 8 rows of V and 32 of K");
+
+  auto compute = [&](int tile, int slot3, const uint16_t* cK, const uint16_t* cV) {
     const int t0 = n0 + tile * KB;
+    // Every K operand of the tile is on its way before the first product, every V
+    // operand before the softmax: LDS answers while the matrix cores and the vector
+    // ALU work.
     f32x16_t st[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) st[mt][i] = 0.0f;
+    {
+      u32x4_t a[MT][KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(cK + swk<D>(mt * 32 + (lane & 31), 2 * ks + hh));
-        st[mt] = mfma32<kBf>(a, qf[ks], st[mt]);
-        if constexpr (kSplitQ) st[mt] = mfma32<kBf>(a, ql[ks], st[mt]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) a[mt][ks] = *reinterpret_cast<const u32x4_t*>(cK + kat[ks] + mt * 32 * D);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[mt][i] = 0.0f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          st[mt] = mfma32<kBf>(a[mt][ks], qf[ks], st[mt]);
+          if constexpr (kSplitQ) st[mt] = mfma32<kBf>(a[mt][ks], ql[ks], st[mt]);
+        }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    const unsigned long long bad = fl->bad[tile % 3];
+    constexpr int TS = KB / 16;
+    short4_t vf[TS][DT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) st[mt] *= qscale;
+    for (int ts = 0; ts < TS; ++ts) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          vf[ts][dt][e] =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(cV + vat[dt] + (ts * 16 + e * 8) * D));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     // This lane's key of slot i is t0 + 4 hh + mt 32 + 8 (i / 4) + i % 4.
-    if (bad != 0) {
+    const unsigned long long bad = fl->bad[slot3];
+    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) {
+      asm volatile("");
       const unsigned long long b = bad >> (4 * hh);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -500,24 +632,25 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[mt][i]);
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__builtin_amdgcn_ballot_w64(mx > m + kLazyRescale) != 0) {
+    const float corr = raise_max<32>(mx, qscale, m);
+    if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
       asm volatile("");
-      const float mn = fmaxf(m, mx);
-      const float corr = mn == -__builtin_inff() ? 1.0f : fast_exp2(m - mn);
-      m = mn;
       l *= corr;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
+      for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= corr;
+      }
     }
     const float negm = m == -__builtin_inff() ? 0.0f : -m;
 #pragma unroll
-    for (int ts = 0; ts < KB / 16; ++ts) {
+    for (int ts = 0; ts < TS; ++ts) {
       uint32_t w[4], wl[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = 8 * (ts & 1) + 2 * j;
-        const float p0 = fast_exp2(st[ts >> 1][i] + negm), p1 = fast_exp2(st[ts >> 1][i + 1] + negm);
+        const float p0 = fast_exp2(fmaf(st[ts >> 1][i], qscale, negm));
+        const float p1 = fast_exp2(fmaf(st[ts >> 1][i + 1], qscale, negm));
         l += p0 + p1;
         w[j] = pack2<kBf>(p0, p1);
         if constexpr (kSplitP) {
@@ -526,15 +659,9 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
         }
       }
       const u32x4_t pb = u32x4_t{w[0], w[1], w[2], w[3]};
-      const int r0 = ts * 16 + 4 * hh + ((lane & 15) >> 2);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const int c = dt * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-        const short4_t a0 =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(cV + swv<D>(r0, c >> 3) + (c & 7)));
-        const short4_t a1 =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(cV + swv<D>(r0 + 8, c >> 3) + (c & 7)));
-        const uint64_t x0 = __builtin_bit_cast(uint64_t, a0), x1 = __builtin_bit_cast(uint64_t, a1);
+        const uint64_t x0 = __builtin_bit_cast(uint64_t, vf[ts][dt][0]), x1 = __builtin_bit_cast(uint64_t, vf[ts][dt][1]);
         const u32x4_t a = u32x4_t{(uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32)};
         o[dt] = mfma32<kBf>(a, pb, o[dt]);
         if constexpr (kSplitP) o[dt] = mfma32<kBf>(a, u32x4_t{wl[0], wl[1], wl[2], wl[3]}, o[dt]);
@@ -542,22 +669,25 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
     }
   };
 
-  int off;
-  int32_t blk = page_at(0, off);
-  issue(0, blk, off);
-  if (ntiles > 1) blk = page_at(1, off);
+  issue(0, 0, sK, sV);
+  if (ntiles > 1) blk = page_at(1);
+  int t3 = 0;  // tile % 3
 #pragma unroll 1
   for (int i = 0; i < ntiles; ++i) {
+    uint16_t* cK = sK + (i & 1) * Sh::TILE;
+    uint16_t* cV = sV + (i & 1) * Sh::TILE;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of tile i
-    finish(i);
+    finish(i, cK, cV);
     __syncthreads();
     asm volatile("" ::: "memory");
-    if (threadIdx.x == 0) fl->bad[(i + 2) % 3] = 0;
+    const int next3 = t3 == 2 ? 0 : t3 + 1;
+    if (threadIdx.x == 0) fl->bad[next3 == 2 ? 0 : next3 + 1] = 0;
     if (i + 1 < ntiles) {
-      issue(i + 1, blk, off);
-      if (i + 2 < ntiles) blk = page_at(i + 2, off);
+      issue(i + 1, next3, sK + ((i + 1) & 1) * Sh::TILE, sV + ((i + 1) & 1) * Sh::TILE);
+      if (i + 2 < ntiles) blk = page_at(i + 2);
     }
-    if (busy) compute(i);
+    if (busy) compute(i, t3, cK, cV);
+    t3 = next3;
   }
 
   // The state of each row.
@@ -577,58 +707,38 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
     }
   }
   __syncthreads();
-  if (fl->odd) restore_odd<KV>(p, u, fl->lim, bmin, KB);
+  if (fl->odd) restore_odd<KV>(p, u, fl->lim, bmin, KB, kSharedWideTile, threadIdx.x, kShThreads);
   __syncthreads();  // (the next piece reuses the tiles and flags)
 }
 
 // ------------------------------------------------------------------- thin --
 
+// One wave's piece; sV: the wave's own LDS tile.
 template <typename KV, bool kBf, int D, bool kSplitQ, bool kSplitP>
-__device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece& u, char* lds, ShFlags* fl,
-                                           float (*s_m)[16], float (*s_l)[16]) {
+__device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece& u, uint16_t* sV, int* s_lim) {
   using Sh = ShShape<D>;
   using Tl = ShTile<KV, kBf>;
-  constexpr int KT = Sh::KT, KS = D / 32, NDT = D / 16, NCH = Sh::NCH, TPD = Sh::TPD, NDMA = Sh::NDMA;
+  constexpr int KT = kSharedThinTile, KS = D / 32, NDT = D / 16, NCH = Sh::NCH, TPD = Sh::TPD, NDMA = Sh::NDMA;
   constexpr int EB = KV::kBytes;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, kg = lane >> 4;
-  uint16_t* sV = reinterpret_cast<uint16_t*>(lds) + wave * KT * D;
-
-  bool live;
-  int64_t qrow;
-  int lim;
-  row_of(p, u, col, live, qrow, lim);
-  u32x4_t qf[KS], ql[kSplitQ ? KS : 1];
-  float back;
-  load_q<kBf, kSplitQ, KS, 32, 16>(p, live, qrow, kg * 8, qf, ql, back);
-  const float qscale = p.qscale * back;
-  int wmin = lim;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) wmin = min(wmin, __shfl_xor(wmin, o, 64));
-  wmin = __builtin_amdgcn_readfirstlane(wmin);
-  if (threadIdx.x < 16) fl->lim[col] = lim;
-  if (threadIdx.x == 0) fl->odd = 0;
-  __syncthreads();
-
   const char* kbase = static_cast<const char*>(p.k) + (int64_t)u.kvh * p.k_sh * EB;
   const char* vbase = static_cast<const char*>(p.v) + (int64_t)u.kvh * p.v_sh * EB;
-  const int n0 = u.first + u.k0 * kSharedTile;
-  const int n1 = min(u.first + u.k1 * kSharedTile, u.end);
-  constexpr int kStep = kShWaves * KT;
-  const int base = n0 + wave * KT;
-  const int ntiles = base < n1 ? (n1 - base + kStep - 1) / kStep : 0;
+  const int n0 = u.first + u.k0 * KT;
+  const int n1 = min(u.first + u.k1 * KT, u.end);
+  const int ntiles = (n1 - n0 + KT - 1) / KT;
 
   // One tile in registers.  Its V is freed into LDS and its K into the scores at the
   // start of a round, and the next tile's loads take their place at once: eight
   // waves of a CU keep 128 KB in flight (D = 128) at half the registers of two tiles.
   typename Tl::Raw tk[2][KS], tv[NDMA];
   const int myrow = lane & 31;
-  auto page_at = [&](int tile, int& off) {
-    const int kk = min(base + tile * kStep + myrow, n1 - 1);
-    const int pg = (int)fastdiv((uint32_t)kk, p.bs_div);
-    off = kk - pg * p.BS;
-    return u.table[pg];
+  auto page_at = [&](int tile) {
+    return u.table[(int)fastdiv((uint32_t)min(n0 + tile * KT + myrow, n1 - 1), p.bs_div)];
+  };
+  auto row_at = [&](int tile, int32_t blk) {
+    const int key = n0 + tile * KT + myrow, kk = min(key, n1 - 1);
+    return key_row(p, blk, kk - (int)fastdiv((uint32_t)kk, p.bs_div) * p.BS, key < n1, EB);
   };
   auto load_k = [&](const ShRow& r) {
 #pragma unroll
@@ -645,31 +755,38 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
       tv[i] = *reinterpret_cast<const typename Tl::Raw*>(vbase + shfl64(r.v, row) + (lane % NCH) * 8 * EB);
     }
   };
+  int32_t blk = page_at(0);
+  bool live;
+  int64_t qrow;
+  int lim;
+  row_of(p, u, col, live, qrow, lim);
+  u32x4_t qf[KS], ql[kSplitQ ? KS : 1];
+  float back;
+  load_q<kBf, kSplitQ, KS, 32, 16>(p, live, qrow, kg * 8, qf, ql, back);
+  ShRow row = row_at(0, blk);
+  load_k(row);
+  load_v(row);
+  if (ntiles > 1) blk = page_at(1);
+  const float qscale = kSplitQ && !kBf ? fmaxf(p.qscale * back, 0x1p-126f) : p.qscale;
+  int wmin = lim;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) wmin = min(wmin, __shfl_xor(wmin, o, 64));
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
 
   float4_t o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   float m = -__builtin_inff(), l = 0.0f;
-
-  int off = 0;
-  int32_t blk = 0;
-  ShRow row;
-  if (ntiles > 0) {
-    blk = page_at(0, off);
-    row = key_row(p, blk, off, base + myrow < n1, EB);
-    load_k(row);
-    load_v(row);
-    if (ntiles > 1) blk = page_at(1, off);
-  }
+  bool odd = false;
 #pragma unroll 1
   for (int i = 0; i < ntiles; ++i) {
-    const int first = base + i * kStep;
+    const int first = n0 + i * KT;
     const uint32_t bad = (uint32_t)__builtin_amdgcn_ballot_w64(row.bad);    // keys on pages outside the cache
     const uint32_t dead = (uint32_t)__builtin_amdgcn_ballot_w64(!row.use);  // keys not used
     const bool masked = first < u.lo || first + KT > wmin;
     const bool more = i + 1 < ntiles;
-    if (more) row = key_row(p, blk, off, first + kStep + myrow < n1, EB);
-    if (i + 2 < ntiles) blk = page_at(i + 2, off);
+    if (more) row = row_at(i + 1, blk);
+    if (i + 2 < ntiles) blk = page_at(i + 2);
     // V to LDS; rows not used are zeroed, what is not finite taken out where a row
     // does not see the whole tile.
 #pragma unroll
@@ -679,8 +796,8 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
       if (dead != 0 || masked) {
         if ((dead >> r) & 1u) {
           x = u32x4_t{0u, 0u, 0u, 0u};
-        } else if (masked && sanitize<kBf>(x)) {
-          fl->odd = 1;
+        } else if (masked) {
+          odd |= sanitize<kBf>(x);
         }
       }
       *reinterpret_cast<u32x4_t*>(sV + r * D + (dm_vpos<D>(r, lane % NCH) << 3)) = x;
@@ -697,7 +814,6 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
         st[mt] = mfma16<kBf>(a, qf[ks], st[mt]);
         if constexpr (kSplitQ) st[mt] = mfma16<kBf>(a, ql[ks], st[mt]);
       }
-      st[mt] *= qscale;
     }
     __builtin_amdgcn_sched_barrier(0);
     if (more) load_k(row);
@@ -713,18 +829,17 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
         }
       }
     }
-    float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
-                     fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__builtin_amdgcn_ballot_w64(mx > m + kLazyRescale) != 0) {
+    const float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
+                           fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+    const float corr = raise_max<16>(mx, qscale, m);
+    if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0) {
       asm volatile("");
-      const float mn = fmaxf(m, mx);
-      const float corr = mn == -__builtin_inff() ? 1.0f : fast_exp2(m - mn);
-      m = mn;
       l *= corr;
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o[dt] *= corr;
+      for (int dt = 0; dt < NDT; ++dt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[dt][e] *= corr;
+      }
     }
     const float negm = m == -__builtin_inff() ? 0.0f : -m;
     uint32_t w[4], wl[4];
@@ -732,7 +847,8 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float p0 = fast_exp2(st[mt][2 * j] + negm), p1 = fast_exp2(st[mt][2 * j + 1] + negm);
+        const float p0 = fast_exp2(fmaf(st[mt][2 * j], qscale, negm));
+        const float p1 = fast_exp2(fmaf(st[mt][2 * j + 1], qscale, negm));
         l += p0 + p1;
         w[mt * 2 + j] = pack2<kBf>(p0, p1);
         if constexpr (kSplitP) {
@@ -757,43 +873,24 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
     }
   }
 
-  // Join the waves' states.
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  __syncthreads();
-  float* s_acc = reinterpret_cast<float*>(lds);  // [waves][16][D]
+  if (live) {
+    const int64_t at = u.slot + col;
 #pragma unroll
-  for (int dt = 0; dt < NDT; ++dt)
-    *reinterpret_cast<float4_t*>(s_acc + (wave * 16 + col) * D + dt * 16 + kg * 4) = o[dt];
-  if (kg == 0) {
-    s_m[wave][col] = m;
-    s_l[wave][col] = l;
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < u.rows * (D / 4); x += kShThreads) {
-    const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
-    float M = -__builtin_inff();
-#pragma unroll
-    for (int w = 0; w < kShWaves; ++w) M = fmaxf(M, s_m[w][r]);
-    float L = 0.0f;
-    float4_t A = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kShWaves; ++w) {
-      const float f = s_m[w][r] == -__builtin_inff() ? (s_l[w][r] != 0.0f ? s_l[w][r] : 0.0f) : fast_exp2(s_m[w][r] - M);
-      L += s_l[w][r] * f;
-      const float4_t a = *reinterpret_cast<const float4_t*>(s_acc + (w * 16 + r) * D + d);
-      if (f != 0.0f) A += a * f;
-    }
-    const int64_t at = u.slot + r;
-    *reinterpret_cast<float4_t*>(p.ws_acc + at * D + d) = A;
-    if (d == 0) {
-      p.ws_m[at] = M;
-      p.ws_l[at] = L;
+    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<float4_t*>(p.ws_acc + at * D + dt * 16 + kg * 4) = o[dt];
+    if (kg == 0) {
+      p.ws_m[at] = m;
+      p.ws_l[at] = l;
     }
   }
-  __syncthreads();
-  if (fl->odd) restore_odd<KV>(p, u, fl->lim, wmin, KT);
-  __syncthreads();
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+    if (lane < 16) s_lim[lane] = lim;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // the states and limits are written
+    __builtin_amdgcn_wave_barrier();
+    restore_odd<KV>(p, u, s_lim, wmin, KT, KT, lane, 64);
+    __builtin_amdgcn_wave_barrier();
+  }
 }
 
 // ----------------------------------------------------------------- kernel --
@@ -803,11 +900,10 @@ __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(D <=
 void shared_kernel(const SharedParams p) {
   __shared__ __attribute__((aligned(16))) char lds[ShShape<D>::LDS];
   __shared__ int32_t s_cum[2 * kSharedMaxSeqs + 1];
+  __shared__ int32_t s_pre[kSharedMaxSeqs];
   __shared__ ShFlags s_fl;
-  __shared__ float s_m[kShWaves][16], s_l[kShWaves][16];
-  __shared__ int s_min[kShWaves];
   int fault;
-  const ShPlan pl = plan_scan(p, s_cum, reinterpret_cast<int32_t*>(lds), fault);
+  const ShPlan pl = plan_scan(p, s_cum, s_pre, reinterpret_cast<int32_t*>(lds), fault);
   const int n = p.NG + p.B;
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) {
@@ -817,60 +913,63 @@ void shared_kernel(const SharedParams p) {
     for (int i = threadIdx.x; i <= n; i += kShThreads) p.ws_meta[2 + i] = fault ? 0 : s_cum[i];
   }
   if (fault) return;
-  const int w = blockIdx.x;
-  int64_t pos = (int64_t)w * pl.share;
-  const int64_t stop = min(pos + pl.share, (int64_t)pl.total);
-  while (pos < stop) {
-    // The entry (group or sequence) that holds `pos`: the last with s_cum <= pos.
-    int lo = 0, hi = n;
+
+  // The piece at `pos` of a stretch that ends at `stop`; pos moves to the unit's end.
+  auto piece = [&](int64_t& pos, int64_t stop, int worker, ShPiece& u) {
+    int lo = 0, hi = n;  // the last entry with s_cum <= pos
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_cum[mid] <= pos) lo = mid; else hi = mid;
     }
     const int entry = __builtin_amdgcn_readfirstlane(lo);
-    ShPiece u;
-    int tiles, rows, blocks;
-    if (entry < p.NG) {
+    const bool prefix = entry < p.NG, thin = !prefix && p.thin;
+    int rows, blocks, tiles;
+    if (prefix) {
       u.b0 = p.group_starts[entry];
       rows = (p.group_starts[entry + 1] - u.b0) * p.SG;
       u.end = prefix_of(p.prefix_lens[entry]);
       u.first = u.lo = 0;
-      tiles = tiles_of(u.end);
+      tiles = wide_tiles(u.end);
       blocks = row_blocks(rows);
     } else {
       u.b0 = entry - p.NG;
-      const int g = group_of(p.group_starts, p.NG, u.b0);
       rows = p.SG;
-      u.lo = g < 0 ? 0 : prefix_of(p.prefix_lens[g]);
+      u.lo = __builtin_amdgcn_readfirstlane(s_pre[u.b0]);
       u.first = own_first(u.lo);
       u.end = p.context_lens[u.b0];
-      tiles = tiles_of(u.end - u.first);
+      tiles = own_tiles(p, u.end - u.first);
       blocks = p.own_rb;
     }
-    const int c = tile_cost(p, rows);
-    const int local = (int)(pos - s_cum[entry]);
-    const int unit = local / (tiles * c);
-    const int64_t begin = (int64_t)s_cum[entry] + (int64_t)unit * tiles * c;  // the unit's place on the line
-    u.k0 = (int)((pos - begin + c - 1) / c);
-    u.k1 = (int)min((int64_t)tiles, (stop - begin + c - 1) / c);
-    pos = begin + (int64_t)tiles * c;
-    if (u.k0 >= u.k1) continue;
+    const int start = thin ? kSharedThinStart : kSharedWideStart, cost = thin ? kSharedThinCost : kSharedWideCost;
+    const int whole = start + tiles * cost, at = __builtin_amdgcn_readfirstlane(s_cum[entry]);
+    const int unit = (int)(pos - at) / whole;
+    const int64_t begin = at + (int64_t)unit * whole;
+    // Tiles that start within the stretch.
+    u.k0 = (int)max((int64_t)0, (pos - begin - start + cost - 1) / cost);
+    u.k1 = (int)min((int64_t)tiles, (stop - begin - start + cost - 1) / cost);
+    pos = begin + whole;
     u.kvh = unit / blocks;
     u.row0 = (unit - u.kvh * blocks) * kSharedWide;
     u.rows = min(rows - u.row0, kSharedWide);
     u.table = p.block_tables + (int64_t)u.b0 * p.bt_stride;
-    if (entry < p.NG) {
-      u.slot = (int64_t)w * kSharedWide + (int64_t)p.HKV * u.b0 * p.SG + (int64_t)u.kvh * rows + u.row0;
-    } else {
-      const int64_t prefix_rows = (int64_t)p.wgs * kSharedWide + (int64_t)p.HKV * p.B * p.SG;
-      u.slot = prefix_rows + (int64_t)w * (p.SG <= kSharedThin ? kSharedThin : kSharedWide) +
-               ((int64_t)u.b0 * p.HKV + u.kvh) * p.SG + u.row0;
-    }
-    if (rows <= kSharedThin)
-      thin_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, lds, &s_fl, s_m, s_l);
-    else
-      wide_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, lds, &s_fl, s_min);
-  }
+    u.slot = prefix ? prefix_slot(p, worker, u.b0, rows, u.kvh, u.row0) : own_slot(p, worker, u.b0, u.kvh, u.row0);
+    return u.k0 < u.k1;
+  };
+
+  ShPiece u;
+  const int64_t wide_end = p.thin ? pl.own : pl.total;
+  int64_t pos = (int64_t)blockIdx.x * pl.share, stop = min(pos + pl.share, wide_end);
+  while (pos < stop)
+    if (piece(pos, stop, blockIdx.x, u)) wide_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, lds, &s_fl);
+  if (!p.thin) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int worker = blockIdx.x * kShWaves + wave, share = pl.share / kShWaves;
+  pos = max((int64_t)worker * share, (int64_t)pl.own);
+  stop = min((int64_t)(worker + 1) * share, (int64_t)pl.total);
+  while (pos < stop)
+    if (piece(pos, stop, worker, u))
+      thin_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, reinterpret_cast<uint16_t*>(lds) + wave * kSharedThinTile * D,
+                                               s_fl.lim + 16 * wave);
 }
 
 template <typename KV, bool kBf, int D>

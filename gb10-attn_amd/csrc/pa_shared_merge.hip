@@ -31,36 +31,35 @@ __global__ __launch_bounds__(64 * kMergeWaves) void shared_merge_kernel(const Sh
   const int keys = ctx - p.S + s + 1;  // that the row attends
   bool bad = p.ws_meta[1] != 0 || ctx > maxctx;
 
-  // The states: n1 of the prefix from row a1 on, n2 of the own keys from a2 on.
-  int n1 = 0, n2 = 0;
+  // The states: n1 of the prefix from workspace row a1 on, n2 of the own keys from a2.
+  int n1 = 0, n2 = 0, step2 = kSharedWide;
   int64_t a1 = 0, a2 = 0;
-  auto pieces = [&](int entry, int unit, int rows, int tiles, int& first) {
-    const int cost = tile_cost(p, rows);
-    const int begin = cum[entry] + unit * tiles * cost;
-    first = begin / share;
-    return (begin + (tiles - 1) * cost) / share - first + 1;
-  };
   if (!bad && keys > 0) {
     const int g = group_of(p.group_starts, p.NG, b);
     const int P = g < 0 ? 0 : prefix_of(p.prefix_lens[g]);
     bad = P > maxctx;
     if (!bad && P > 0) {
       const int b0 = p.group_starts[g], rows = (p.group_starts[g + 1] - b0) * p.SG;
-      const int at = (b - b0) * p.SG + mine;
+      const int at = (b - b0) * p.SG + mine, tiles = wide_tiles(P);
+      const int unit = kvh * row_blocks(rows) + at / kSharedWide;
       int first;
-      n1 = pieces(g, kvh * row_blocks(rows) + at / kSharedWide, rows, tiles_of(P), first);
-      a1 = (int64_t)first * kSharedWide + (int64_t)p.HKV * b0 * p.SG + (int64_t)kvh * rows + at;
+      unit_workers(cum[g] + unit * wide_cost(tiles), kSharedWideStart, kSharedWideCost, tiles, share, first, n1);
+      a1 = prefix_slot(p, first, b0, rows, kvh, at);
     }
     if (!bad && ctx > P) {
+      const int tiles = own_tiles(p, ctx - own_first(P));
+      const int unit = kvh * p.own_rb + mine / kSharedWide, begin = cum[p.NG + b] + unit * own_cost(p, tiles);
       int first;
-      n2 = pieces(p.NG + b, kvh * p.own_rb + mine / kSharedWide, p.SG, tiles_of(ctx - own_first(P)), first);
-      const int step = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
-      a2 = (int64_t)p.wgs * kSharedWide + (int64_t)p.HKV * p.B * p.SG + (int64_t)first * step +
-           ((int64_t)b * p.HKV + kvh) * p.SG + mine;
+      if (p.thin) {
+        unit_workers(begin, kSharedThinStart, kSharedThinCost, tiles, share / kShWaves, first, n2);
+        step2 = kSharedThin;
+      } else {
+        unit_workers(begin, kSharedWideStart, kSharedWideCost, tiles, share, first, n2);
+      }
+      a2 = own_slot(p, first, b, kvh, mine);
     }
   }
-  const int step1 = kSharedWide, step2 = p.SG <= kSharedThin ? kSharedThin : kSharedWide;
-  auto place = [&](int i) { return i < n1 ? a1 + (int64_t)i * step1 : a2 + (int64_t)(i - n1) * step2; };
+  auto place = [&](int i) { return i < n1 ? a1 + (int64_t)i * kSharedWide : a2 + (int64_t)(i - n1) * step2; };
   const int all = n1 + n2;
   float M = -__builtin_inff();
   for (int i0 = 0; i0 < all; i0 += 64)
