@@ -1585,8 +1585,8 @@ extern "C" int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, cons
 // per CU, one at D = 256), or has as many as the keys that the tables can hold make
 // shares of.
 static int plan_shared(SharedParams* p) {
-  if (p->B > kSharedMaxSeqs || p->NG > kSharedMaxSeqs)
-    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups", kSharedMaxSeqs);
+  if (p->B > kSharedMaxSeqs || p->NG > kSharedMaxGroups)
+    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and %d groups", kSharedMaxSeqs, kSharedMaxGroups);
   int cus = 0, rc;
   if ((rc = device_cu_count(&cus))) return rc;
   const int64_t sg = (int64_t)p->S * p->G, rows = p->B * sg;
@@ -1601,6 +1601,7 @@ static int plan_shared(SharedParams* p) {
   const int64_t thin = kSharedThinStart + kSharedThinCost * ((keys + kSharedThinTile - 1) / kSharedThinTile);
   const int64_t units = p->HKV * (rows / kSharedWide + p->NG), own = (int64_t)p->HKV * p->B * p->own_rb;
   const double most = (double)units * (double)wide + (double)own * (double)(p->thin ? thin : wide);
+  // (The last work-group's stretch may end past the line.)
   if (most >= (double)(1LL << 31) - 1e6) return fail(PA_ERR_UNSUPPORTED, "too many keys and query rows for one call");
   p->wgs = (int32_t)std::min<int64_t>((p->D <= 128 ? 2 : 1) * (int64_t)cus, (int64_t)most / kSharedMinShare + 1);
   p->sg_div = make_fastdiv((uint32_t)std::max(1, p->SG));
@@ -1634,9 +1635,10 @@ extern "C" size_t paged_attention_shared_prefix_workspace_size(const pa_tensor_t
     fail(PA_ERR_INVALID_ARGUMENT, "group_starts must have at least one entry");
     return (size_t)-1;
   }
-  if (q->shape[0] > kSharedMaxSeqs || S >= (1LL << 31) || group_starts->shape[0] > kSharedMaxSeqs + 1 ||
+  if (q->shape[0] > kSharedMaxSeqs || S >= (1LL << 31) || group_starts->shape[0] > kSharedMaxGroups + 1 ||
       k_cache->shape[1] >= (1LL << 31) || block_tables->shape[1] * k_cache->shape[1] >= (1LL << 31)) {
-    fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups, and 32-bit token indices", kSharedMaxSeqs);
+    fail(PA_ERR_UNSUPPORTED, "at most %d sequences and %d groups, and 32-bit token indices", kSharedMaxSeqs,
+         kSharedMaxGroups);
     return (size_t)-1;
   }
   SharedParams p;
@@ -1678,8 +1680,8 @@ extern "C" int paged_attention_shared_prefix(pa_tensor_t* out, const pa_tensor_t
   if ((rc = check_index(group_starts, "group_starts", -1, false))) return rc;
   if (group_starts->shape[0] < 1) return fail(PA_ERR_INVALID_ARGUMENT, "group_starts must have at least one entry");
   if ((rc = check_index(prefix_lens, "prefix_lens", group_starts->shape[0] - 1, false))) return rc;
-  if (group_starts->shape[0] > kSharedMaxSeqs + 1)
-    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and groups", kSharedMaxSeqs);
+  if (group_starts->shape[0] > kSharedMaxGroups + 1)
+    return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and %d groups", kSharedMaxSeqs, kSharedMaxGroups);
   const DecodeParams& d = a.p;
   if ((int64_t)d.B * d.Sq * d.H == 0) return PA_OK;
   if (!aligned16(q->data)) return fail(PA_ERR_UNSUPPORTED, "shared prefixes need a 16-byte aligned q");

@@ -341,6 +341,7 @@ constexpr int kSharedWideCost = 4, kSharedWideStart = 8;
 constexpr int kSharedThinCost = 3, kSharedThinStart = 2;
 constexpr int kSharedMinShare = 4 * kSharedThinCost;  // a wave's share holds the start of a tile
 constexpr int kSharedMaxSeqs = 1024;
+constexpr int kSharedMaxGroups = 512;
 
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = 64 * kDecodeWaves;

@@ -47,6 +47,18 @@ namespace pa {
 constexpr int kShThreads = 256;
 constexpr int kShWaves = 4;
 
+// 16 bytes per lane straight to LDS byte address `to` (wave-uniform) + 16 lane, from a
+// uniform base and a 32-bit lane offset, or from a lane's address.  The compiler does not
+// see the loads: the caller waits for vmcnt before the barrier that publishes the data.
+// (A spilled lane address cost a wait for every earlier load; the scalar base leaves
+// one register a load.)
+__device__ inline void dma_at(const char* base, uint32_t off, uint32_t to) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(to));
+}
+__device__ inline void dma_at(const char* from, uint32_t to) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(to));
+}
+
 // Tile type of a cache: FP8 codes widen to fp16 or bf16.
 template <typename KV, bool kBf>
 struct ShTile {
@@ -105,7 +117,8 @@ struct ShPlan {
 };
 
 // A sequence's group, or -1.  starts: [NG + 1], non-decreasing.
-__device__ inline int group_of(const int32_t* starts, int NG, int b) {
+template <typename T>
+__device__ inline int group_of(const T* starts, int NG, int b) {
   if (b < starts[0] || b >= starts[NG]) return -1;
   int lo = 0, hi = NG;  // last g with starts[g] <= b
   while (hi - lo > 1) {
@@ -130,20 +143,27 @@ __device__ inline int own_first(int prefix) { return prefix & ~15; }
 // Prefix of a group as attended: none where it is negative.
 __device__ inline int prefix_of(int n) { return n > 0 ? n : 0; }
 
-// Where the units lie on the line: s_cum[i] is the cost before entry i (groups, then
-// sequences), s_pre[b] the prefix of sequence b.  s_tmp: scratch of 2 NG + 1 + 8
-// words.  Every thread of the work-group; fault: the group starts are unusable.
-__device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_t* s_pre, int32_t* s_tmp, int& fault) {
+// What a work-group knows of the batch: where the units lie on the line, and each
+// sequence's prefix and context.
+struct ShTables {
+  int32_t cum[kSharedMaxGroups + kSharedMaxSeqs + 1];  // cost before entry i: groups, then sequences
+  int32_t pre[kSharedMaxSeqs];                         // prefix of the sequence's group, 0: none
+  int32_t ctx[kSharedMaxSeqs];
+  uint16_t start[kSharedMaxGroups + 2];                // first sequence of each group, and the end
+};
+
+// Fills the tables.  s_tmp: scratch of NG + 8 words.  Every thread of the work-group;
+// fault: the group starts are unusable.
+__device__ inline ShPlan plan_scan(const SharedParams& p, ShTables& s, int32_t* s_tmp, int& fault) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int32_t* s_start = s_tmp + 8;
-  int32_t* s_len = s_start + p.NG + 1;
+  int32_t* s_len = s_tmp + 8;
   const int maxctx = p.MB * p.BS;
-  int ctx = tid < p.B ? p.context_lens[tid] : 0;  // (in flight beside the groups)
   int bad = 0;
+  for (int b = tid; b < p.B; b += kShThreads) s.ctx[b] = p.context_lens[b];
   for (int g = tid; g <= p.NG; g += kShThreads) {
     const int a = p.group_starts[g];
     bad |= a < 0 || a > p.B || (g > 0 && p.group_starts[g - 1] > a);
-    s_start[g] = a;
+    s.start[g] = (uint16_t)a;
     if (g < p.NG) s_len[g] = prefix_of(p.prefix_lens[g]);
   }
   fault = __syncthreads_or(bad);
@@ -171,26 +191,35 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, int32_t* s_cum, int32_
     const int g = i0 + tid;
     int c = 0;
     if (g < p.NG && s_len[g] > 0 && s_len[g] <= maxctx)
-      c = p.HKV * row_blocks((s_start[g + 1] - s_start[g]) * p.SG) * wide_cost(wide_tiles(s_len[g]));
-    scan(g, p.NG, c, s_cum);
+      c = p.HKV * row_blocks((s.start[g + 1] - s.start[g]) * p.SG) * wide_cost(wide_tiles(s_len[g]));
+    scan(g, p.NG, c, s.cum);
   }
   const int own = carry;
   for (int i0 = 0; i0 < p.B; i0 += kShThreads) {
     const int b = i0 + tid;
     int c = 0;
     if (b < p.B) {
-      if (i0 > 0) ctx = p.context_lens[b];
-      const int g = group_of(s_start, p.NG, b);
-      const int P = g < 0 ? 0 : s_len[g];
-      s_pre[b] = P;
+      const int g = group_of(s.start, p.NG, b);
+      const int P = g < 0 ? 0 : s_len[g], ctx = s.ctx[b];
+      s.pre[b] = P;
       if (ctx > P && ctx <= maxctx) c = p.HKV * p.own_rb * own_cost(p, own_tiles(p, ctx - own_first(P)));
     }
-    scan(b, p.B, c, s_cum + p.NG);
+    scan(b, p.B, c, s.cum + p.NG);
   }
-  if (tid == 0) s_cum[p.NG + p.B] = carry;
+  if (tid == 0) s.cum[p.NG + p.B] = carry;
   __syncthreads();
   const int even = (carry + p.wgs - 1) / p.wgs;
   return {carry, own, max(kSharedMinShare, (even + 3) & ~3)};
+}
+
+// The last entry that begins at or before `pos` of the line, by 64-way search.
+__device__ inline int entry_at(const ShTables& s, int n, int pos) {
+  const int lane = threadIdx.x & 63, step = (n + 63) / 64;
+  const int i = lane * step;
+  const int block = __builtin_popcountll(__builtin_amdgcn_ballot_w64(i < n && s.cum[min(i, n)] <= pos)) - 1;
+  const int j = block * step + lane;
+  return block * step +
+         __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < step && j < n && s.cum[min(j, n)] <= pos)) - 1;
 }
 
 // Which states a unit left: workers first .. last, for tiles of `cost` behind `start`
@@ -232,7 +261,8 @@ struct ShPiece {
 
 // Row `r` of a piece: its q row (index of [B, S, H]) and the end of the keys it
 // attends; a row past the block attends whatever is there (it is not written).
-__device__ inline void row_of(const SharedParams& p, const ShPiece& u, int r, bool& live, int64_t& qrow, int& lim) {
+__device__ inline void row_of(const SharedParams& p, const ShPiece& u, const ShTables& tab, int r, bool& live,
+                              int64_t& qrow, int& lim) {
   live = r < u.rows;
   const uint32_t R = (uint32_t)(u.row0 + (live ? r : 0));
   const uint32_t i = fastdiv(R, p.sg_div);
@@ -240,7 +270,7 @@ __device__ inline void row_of(const SharedParams& p, const ShPiece& u, int r, bo
   const uint32_t s = fastdiv(t, p.g_div);
   const int b = u.b0 + (int)i;
   qrow = ((int64_t)b * p.S + s) * p.H + (int64_t)u.kvh * p.G + (t - s * (uint32_t)p.G);
-  const int ctx = max(p.context_lens[b], 0);
+  const int ctx = max(tab.ctx[b], 0);
   const int n = ctx <= p.MB * p.BS ? min(ctx - p.S + (int)s + 1, u.end) : 0;
   lim = live ? n : 0x7fffffff;
 }
@@ -345,7 +375,7 @@ struct ShShape {
   static constexpr int NDMA = kSharedThinTile / TPD;  // V loads of a thin tile
   static constexpr int LDS_WIDE = 4 * TILE * 2;       // K and V, two tiles
   static constexpr int LDS_THIN = kShWaves * kSharedThinTile * D * 2;
-  static constexpr int LDS_PLAN = (8 + 2 * kSharedMaxSeqs + 1) * 4;
+  static constexpr int LDS_PLAN = (8 + kSharedMaxGroups) * 4;
   static constexpr int LDS_BODY = LDS_WIDE > LDS_THIN ? LDS_WIDE : LDS_THIN;
   static constexpr int LDS = LDS_BODY > LDS_PLAN ? LDS_BODY : LDS_PLAN;
   static_assert(NP >= 1 && RPW % TPD == 0, "tile shape");
@@ -400,7 +430,8 @@ __device__ inline float raise_max(float mx, float qscale, float& m) {
 // ------------------------------------------------------------------- wide --
 
 template <typename KV, bool kBf, int D, bool kSplitQ, bool kSplitP>
-__device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece& u, char* lds, ShFlags* fl) {
+__device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece& u, const ShTables& s,
+                                           char* lds, ShFlags* fl) {
   using Sh = ShShape<D>;
   using Tl = ShTile<KV, kBf>;
   constexpr int KB = Sh::KB, MT = Sh::MT, KS = Sh::KS, DT = Sh::DT, NCH = Sh::NCH, TPD = Sh::TPD, RPW = Sh::RPW,
@@ -438,7 +469,7 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   bool live;
   int64_t qrow;
   int lim;
-  row_of(p, u, wave * 32 + (lane & 31), live, qrow, lim);
+  row_of(p, u, s, wave * 32 + (lane & 31), live, qrow, lim);
   const bool busy = wave * 32 < u.rows;
   u32x4_t qf[KS], ql[kSplitQ ? KS : 1];
   float back;
@@ -460,7 +491,9 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
 
   uint32_t dead = 0;  // bit i: this lane's row of load i is not used
   typename Tl::Raw kr[Tl::kF8 ? NP : 1], vr[Tl::kF8 ? NP : 1];
-  auto issue = [&](int tile, int slot3, uint16_t* dK, uint16_t* dV) {
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)lds + wave * (RPW * D * 2);
+  auto issue = [&](int tile, int slot3) {
+    const uint32_t toK = lds0 + (tile & 1) * (Sh::TILE * 2), toV = toK + 2 * Sh::TILE * 2;
     const int key = n0 + tile * KB + wave * RPW;  // first of this wave's rows
     dead = 0;
     if (p.page16) {
@@ -484,8 +517,8 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
           kr[i] = *reinterpret_cast<const typename Tl::Raw*>(ka + klane[i]);
           vr[i] = *reinterpret_cast<const typename Tl::Raw*>(va + vlane[i]);
         } else {
-          lds_dma16_async(ka + klane[i], (lds_void_t*)(dK + wave * RPW * D + i * 512));
-          lds_dma16_async(va + vlane[i], (lds_void_t*)(dV + wave * RPW * D + i * 512));
+          dma_at(ka, klane[i], toK + i * 1024);
+          dma_at(va, vlane[i], toV + i * 1024);
         }
       }
     } else {
@@ -503,8 +536,8 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
           kr[i] = *reinterpret_cast<const typename Tl::Raw*>(ka);
           vr[i] = *reinterpret_cast<const typename Tl::Raw*>(va);
         } else {
-          lds_dma16_async(ka, (lds_void_t*)(dK + wave * RPW * D + i * 512));
-          lds_dma16_async(va, (lds_void_t*)(dV + wave * RPW * D + i * 512));
+          dma_at(ka, toK + i * 1024);
+          dma_at(va, toV + i * 1024);
         }
       }
     }
@@ -546,61 +579,58 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   }
   float m = -__builtin_inff(), l = 0.0f;
 
-  // LDS addresses of the operands: K chunk of k-step ks (m-tiles 32 rows apart), V of
-  // dim tile dt (16-key steps 16 rows apart, the operand's second half 8).
-  int kat[KS], vat[DT];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) kat[ks] = swk<D>(lane & 31, 2 * ks + hh);
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int c = dt * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    vat[dt] = swv<D>(4 * hh + ((lane & 15) >> 2), c >> 3) + (c & 7);
-  }
+  // LDS places of the operands: the swizzles flip bits of the chunk number, so K's
+  // k-step ks is ks * 16 elements away by exclusive or, V's dim tile dt dt * 32; m-tiles
+  // of K lie 32 rows apart, 16-key steps of V 16 rows, an operand's second half 8.
+  const int kat = swk<D>(lane & 31, hh);
+  const int vat = swv<D>(4 * hh + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) + (lane & 1) * 4;
   static_assert(((8 >> PfShape<D>::VSH) & PfShape<D>::VSW) == 0 && ((16 >> PfShape<D>::VSH) & PfShape<D>::VSW) == 0 &&
                     ((32 >> PfShape<D>::KSH) & PfShape<D>::KSW) == 0,
                 "the swizzles repeat every 8 rows of V and 32 of K");
 
   auto compute = [&](int tile, int slot3, const uint16_t* cK, const uint16_t* cV) {
     const int t0 = n0 + tile * KB;
-    // Every K operand of the tile is on its way before the first product, every V
-    // operand before the softmax: LDS answers while the matrix cores and the vector
-    // ALU work.
+    // K operands are read four k-steps ahead of their products and V operands two key
+    // steps ahead (the first before the softmax), so that LDS answers while the matrix
+    // cores and the vector ALU work.  (All of them ahead spilled at D = 128.)
+    constexpr int WK = KS < 4 ? KS : 4, TS = KB / 16;
     f32x16_t st[MT];
-    {
-      u32x4_t a[MT][KS];
+    u32x4_t a[WK][MT];
+    auto load_a = [&](int ks) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) a[mt][ks] = *reinterpret_cast<const u32x4_t*>(cK + kat[ks] + mt * 32 * D);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[mt][i] = 0.0f;
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          st[mt] = mfma32<kBf>(a[mt][ks], qf[ks], st[mt]);
-          if constexpr (kSplitQ) st[mt] = mfma32<kBf>(a[mt][ks], ql[ks], st[mt]);
-        }
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    constexpr int TS = KB / 16;
-    short4_t vf[TS][DT][2];
-#pragma unroll
-    for (int ts = 0; ts < TS; ++ts) {
+      for (int mt = 0; mt < MT; ++mt)
+        a[ks % WK][mt] = *reinterpret_cast<const u32x4_t*>(cK + (kat ^ (ks * 16)) + mt * 32 * D);
+    };
+    short4_t vf[2][DT][2];
+    auto load_vf = [&](int ts) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          vf[ts][dt][e] =
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t*)(cV + vat[dt] + (ts * 16 + e * 8) * D));
+          vf[ts & 1][dt][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_short4_t*)(cV + (vat ^ (dt * 32)) + (ts * 16 + e * 8) * D));
       }
+    };
+#pragma unroll
+    for (int ks = 0; ks < WK; ++ks) load_a(ks);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[mt][i] = 0.0f;
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        st[mt] = mfma32<kBf>(a[ks % WK][mt], qf[ks], st[mt]);
+        if constexpr (kSplitQ) st[mt] = mfma32<kBf>(a[ks % WK][mt], ql[ks], st[mt]);
+      }
+      if (ks + WK < KS) load_a(ks + WK);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    load_vf(0);
+    if constexpr (TS > 1) load_vf(1);
     __builtin_amdgcn_sched_barrier(0);
     // This lane's key of slot i is t0 + 4 hh + mt 32 + 8 (i / 4) + i % 4.
     const unsigned long long bad = fl->bad[slot3];
@@ -661,15 +691,18 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
       const u32x4_t pb = u32x4_t{w[0], w[1], w[2], w[3]};
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const uint64_t x0 = __builtin_bit_cast(uint64_t, vf[ts][dt][0]), x1 = __builtin_bit_cast(uint64_t, vf[ts][dt][1]);
-        const u32x4_t a = u32x4_t{(uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32)};
-        o[dt] = mfma32<kBf>(a, pb, o[dt]);
-        if constexpr (kSplitP) o[dt] = mfma32<kBf>(a, u32x4_t{wl[0], wl[1], wl[2], wl[3]}, o[dt]);
+        const uint64_t x0 = __builtin_bit_cast(uint64_t, vf[ts & 1][dt][0]),
+                       x1 = __builtin_bit_cast(uint64_t, vf[ts & 1][dt][1]);
+        const u32x4_t av = u32x4_t{(uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32)};
+        o[dt] = mfma32<kBf>(av, pb, o[dt]);
+        if constexpr (kSplitP) o[dt] = mfma32<kBf>(av, u32x4_t{wl[0], wl[1], wl[2], wl[3]}, o[dt]);
       }
+      if (ts + 2 < TS) load_vf(ts + 2);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  issue(0, 0, sK, sV);
+  issue(0, 0);
   if (ntiles > 1) blk = page_at(1);
   int t3 = 0;  // tile % 3
 #pragma unroll 1
@@ -683,7 +716,7 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
     const int next3 = t3 == 2 ? 0 : t3 + 1;
     if (threadIdx.x == 0) fl->bad[next3 == 2 ? 0 : next3 + 1] = 0;
     if (i + 1 < ntiles) {
-      issue(i + 1, next3, sK + ((i + 1) & 1) * Sh::TILE, sV + ((i + 1) & 1) * Sh::TILE);
+      issue(i + 1, next3);
       if (i + 2 < ntiles) blk = page_at(i + 2);
     }
     if (busy) compute(i, t3, cK, cV);
@@ -715,7 +748,8 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
 
 // One wave's piece; sV: the wave's own LDS tile.
 template <typename KV, bool kBf, int D, bool kSplitQ, bool kSplitP>
-__device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece& u, uint16_t* sV, int* s_lim) {
+__device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece& u, const ShTables& s,
+                                           uint16_t* sV, int* s_lim) {
   using Sh = ShShape<D>;
   using Tl = ShTile<KV, kBf>;
   constexpr int KT = kSharedThinTile, KS = D / 32, NDT = D / 16, NCH = Sh::NCH, TPD = Sh::TPD, NDMA = Sh::NDMA;
@@ -759,7 +793,7 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
   bool live;
   int64_t qrow;
   int lim;
-  row_of(p, u, col, live, qrow, lim);
+  row_of(p, u, s, col, live, qrow, lim);
   u32x4_t qf[KS], ql[kSplitQ ? KS : 1];
   float back;
   load_q<kBf, kSplitQ, KS, 32, 16>(p, live, qrow, kg * 8, qf, ql, back);
@@ -899,56 +933,56 @@ template <typename KV, bool kBf, int D, bool kSplitQ, bool kSplitP>
 __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1)))
 void shared_kernel(const SharedParams p) {
   __shared__ __attribute__((aligned(16))) char lds[ShShape<D>::LDS];
-  __shared__ int32_t s_cum[2 * kSharedMaxSeqs + 1];
-  __shared__ int32_t s_pre[kSharedMaxSeqs];
+  __shared__ ShTables s_tab;
   __shared__ ShFlags s_fl;
   int fault;
-  const ShPlan pl = plan_scan(p, s_cum, s_pre, reinterpret_cast<int32_t*>(lds), fault);
+  const ShPlan pl = plan_scan(p, s_tab, reinterpret_cast<int32_t*>(lds), fault);
   const int n = p.NG + p.B;
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) {
       p.ws_meta[0] = pl.share;
       p.ws_meta[1] = fault;
     }
-    for (int i = threadIdx.x; i <= n; i += kShThreads) p.ws_meta[2 + i] = fault ? 0 : s_cum[i];
+    for (int i = threadIdx.x; i <= n; i += kShThreads) p.ws_meta[2 + i] = fault ? 0 : s_tab.cum[i];
   }
   if (fault) return;
 
   // The piece at `pos` of a stretch that ends at `stop`; pos moves to the unit's end.
-  auto piece = [&](int64_t& pos, int64_t stop, int worker, ShPiece& u) {
-    int lo = 0, hi = n;  // the last entry with s_cum <= pos
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_cum[mid] <= pos) lo = mid; else hi = mid;
-    }
-    const int entry = __builtin_amdgcn_readfirstlane(lo);
+  auto piece = [&](int& pos, int stop, int worker, ShPiece& u) {
+    const int entry = __builtin_amdgcn_readfirstlane(entry_at(s_tab, n, pos));
     const bool prefix = entry < p.NG, thin = !prefix && p.thin;
     int rows, blocks, tiles;
     if (prefix) {
-      u.b0 = p.group_starts[entry];
-      rows = (p.group_starts[entry + 1] - u.b0) * p.SG;
-      u.end = prefix_of(p.prefix_lens[entry]);
+      u.b0 = __builtin_amdgcn_readfirstlane(s_tab.start[entry]);
+      rows = (__builtin_amdgcn_readfirstlane(s_tab.start[entry + 1]) - u.b0) * p.SG;
+      u.end = __builtin_amdgcn_readfirstlane(s_tab.pre[u.b0]);
       u.first = u.lo = 0;
       tiles = wide_tiles(u.end);
       blocks = row_blocks(rows);
     } else {
       u.b0 = entry - p.NG;
       rows = p.SG;
-      u.lo = __builtin_amdgcn_readfirstlane(s_pre[u.b0]);
+      u.lo = __builtin_amdgcn_readfirstlane(s_tab.pre[u.b0]);
       u.first = own_first(u.lo);
-      u.end = p.context_lens[u.b0];
+      u.end = __builtin_amdgcn_readfirstlane(s_tab.ctx[u.b0]);
       tiles = own_tiles(p, u.end - u.first);
       blocks = p.own_rb;
     }
-    const int start = thin ? kSharedThinStart : kSharedWideStart, cost = thin ? kSharedThinCost : kSharedWideCost;
-    const int whole = start + tiles * cost, at = __builtin_amdgcn_readfirstlane(s_cum[entry]);
-    const int unit = (int)(pos - at) / whole;
-    const int64_t begin = at + (int64_t)unit * whole;
+    const int start = thin ? kSharedThinStart : kSharedWideStart;
+    const int whole = thin ? kSharedThinStart + tiles * kSharedThinCost : wide_cost(tiles);
+    const int at = __builtin_amdgcn_readfirstlane(s_tab.cum[entry]);
+    const int unit = (int)((uint32_t)(pos - at) / (uint32_t)whole);
+    const int begin = at + unit * whole;
     // Tiles that start within the stretch.
-    u.k0 = (int)max((int64_t)0, (pos - begin - start + cost - 1) / cost);
-    u.k1 = (int)min((int64_t)tiles, (stop - begin - start + cost - 1) / cost);
+    auto tile_from = [&](int x) {
+      const uint32_t d = (uint32_t)max(x - begin - start, 0);
+      return (int)min(thin ? (d + kSharedThinCost - 1) / kSharedThinCost : (d + kSharedWideCost - 1) / kSharedWideCost,
+                      (uint32_t)tiles);
+    };
+    u.k0 = tile_from(pos);
+    u.k1 = tile_from(stop);
     pos = begin + whole;
-    u.kvh = unit / blocks;
+    u.kvh = blocks == 1 ? unit : (int)((uint32_t)unit / (uint32_t)blocks);
     u.row0 = (unit - u.kvh * blocks) * kSharedWide;
     u.rows = min(rows - u.row0, kSharedWide);
     u.table = p.block_tables + (int64_t)u.b0 * p.bt_stride;
@@ -957,18 +991,18 @@ void shared_kernel(const SharedParams p) {
   };
 
   ShPiece u;
-  const int64_t wide_end = p.thin ? pl.own : pl.total;
-  int64_t pos = (int64_t)blockIdx.x * pl.share, stop = min(pos + pl.share, wide_end);
+  const int wide_end = p.thin ? pl.own : pl.total;
+  int pos = blockIdx.x * pl.share, stop = min(pos + pl.share, wide_end);
   while (pos < stop)
-    if (piece(pos, stop, blockIdx.x, u)) wide_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, lds, &s_fl);
+    if (piece(pos, stop, blockIdx.x, u)) wide_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, s_tab, lds, &s_fl);
   if (!p.thin) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = blockIdx.x * kShWaves + wave, share = pl.share / kShWaves;
-  pos = max((int64_t)worker * share, (int64_t)pl.own);
-  stop = min((int64_t)(worker + 1) * share, (int64_t)pl.total);
+  pos = max(worker * share, pl.own);
+  stop = min((worker + 1) * share, pl.total);
   while (pos < stop)
     if (piece(pos, stop, worker, u))
-      thin_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, reinterpret_cast<uint16_t*>(lds) + wave * kSharedThinTile * D,
+      thin_piece<KV, kBf, D, kSplitQ, kSplitP>(p, u, s_tab, reinterpret_cast<uint16_t*>(lds) + wave * kSharedThinTile * D,
                                                s_fl.lim + 16 * wave);
 }
 

@@ -214,7 +214,7 @@ def shared_call(pa, a, scale=0.1, ks=1.0, vs=1.0, ws=FAKE, size=1 << 40):
     (dict(H=9), {}, 1, "n_head must be divisible by n_kv_head"),
     (dict(D=96), {}, 2, "unsupported head_dim 96"),
     (dict(B=1025), {}, 2, "at most 1024 sequences"),
-    (dict(NG=1025), {}, 2, "at most 1024 sequences"),
+    (dict(NG=513), {}, 2, "at most 1024 sequences and 512 groups"),
     ({}, dict(starts=([3], I64)), 1, "group_starts must be int32"),
     ({}, dict(starts=([0], I32), prefix=([0], I32)), 1, "group_starts must have at least one entry"),
     ({}, dict(prefix=([3], I32)), 1, "prefix_lens must have 2 entries"),
@@ -245,6 +245,6 @@ def test_shared_prefix_scalars_and_null(pa):
     assert shared_call(pa, shared_args(pa, B=0), ws=None, size=0) == 0
     assert shared_call(pa, shared_args(pa, S=0), ws=None, size=0) == 0
     size = pa.lib().paged_attention_shared_prefix_workspace_size
-    for sizes in (dict(B=1025), dict(NG=1025), dict(H=9), dict(D=512)):
+    for sizes in (dict(B=1025), dict(NG=513), dict(H=9), dict(D=512)):
         b = shared_args(pa, **sizes)
         assert size(*refs(b[n] for n in ("q", "k", "bt", "starts"))) == C.c_size_t(-1).value
