@@ -1609,7 +1609,9 @@ static int plan_shared(SharedParams* p) {
   return PA_OK;
 }
 
-static size_t shared_meta_bytes(const SharedParams& p) { return (4 * (size_t)(3 + p.NG + p.B) + 255) & ~(size_t)255; }
+static size_t shared_meta_bytes(const SharedParams& p) {
+  return (4 * (size_t)(8 + kSharedMeta * p.B) + 255) & ~(size_t)255;
+}
 static size_t shared_rows(const SharedParams& p) {
   return (size_t)p.wgs * (kSharedWide + (p.thin ? 4 * kSharedThin : kSharedWide)) + 2 * (size_t)p.HKV * p.B * p.SG;
 }

@@ -325,8 +325,8 @@ struct SharedParams {
   float q_sign;           // its sign, or 0, applied to q
   uint32_t q_and, q_xor;  // the same on packed 16-bit q: bits & q_and ^ q_xor
   float vscale;
-  // Workspace: share, fault and the cost sums; the pieces' softmax states.
-  int32_t* ws_meta;  // [2 + NG + 1 + B + 1]
+  // Workspace: what the merge needs of the plan, and the pieces' softmax states.
+  int32_t* ws_meta;  // share, fault, 6 unused; kSharedMeta words a sequence
   float* ws_acc;     // [rows][D]
   float* ws_m;       // [rows] log2 units
   float* ws_l;       // [rows]
@@ -336,10 +336,12 @@ constexpr int kSharedThin = 16;       // ... of a thin one
 constexpr int kSharedWideTile = 64;   // keys of a tile of either
 constexpr int kSharedThinTile = 32;
 // Cost of a tile and of a unit's start, in the parts that are shared out (about
-// 0.3 us of a work-group; a thin tile is a wave's, four at a time).
-constexpr int kSharedWideCost = 4, kSharedWideStart = 8;
+// 0.4 us of a work-group; a thin tile is a wave's, four at a time).
+constexpr int kSharedWideCost = 7, kSharedWideStart = 10;
 constexpr int kSharedThinCost = 3, kSharedThinStart = 2;
 constexpr int kSharedMinShare = 4 * kSharedThinCost;  // a wave's share holds the start of a tile
+constexpr int kSharedMeta = 8;  // prefix, context, the group's first sequence, its rows, cost before its units
+                                // and before the sequence's own
 constexpr int kSharedMaxSeqs = 1024;
 constexpr int kSharedMaxGroups = 512;
 

@@ -158,14 +158,21 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, ShTables& s, int32_t* 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int32_t* s_len = s_tmp + 8;
   const int maxctx = p.MB * p.BS;
+  // (The first round's loads are all in flight before any is used.)
   int bad = 0;
-  for (int b = tid; b < p.B; b += kShThreads) s.ctx[b] = p.context_lens[b];
-  for (int g = tid; g <= p.NG; g += kShThreads) {
-    const int a = p.group_starts[g];
-    bad |= a < 0 || a > p.B || (g > 0 && p.group_starts[g - 1] > a);
+  const bool own0 = tid < p.B, end0 = tid <= p.NG, len0 = tid < p.NG;
+  const int c0 = own0 ? p.context_lens[tid] : 0, a0 = end0 ? p.group_starts[tid] : 0;
+  const int b0 = len0 ? p.group_starts[tid + 1] : 0, l0 = len0 ? p.prefix_lens[tid] : 0;
+  auto group = [&](int g, int a, int next, int len) {
+    bad |= a < 0 || a > p.B || (g < p.NG && next < a);
     s.start[g] = (uint16_t)a;
-    if (g < p.NG) s_len[g] = prefix_of(p.prefix_lens[g]);
-  }
+    if (g < p.NG) s_len[g] = prefix_of(len);
+  };
+  if (own0) s.ctx[tid] = c0;
+  if (end0) group(tid, a0, b0, l0);
+  for (int b = tid + kShThreads; b < p.B; b += kShThreads) s.ctx[b] = p.context_lens[b];
+  for (int g = tid + kShThreads; g <= p.NG; g += kShThreads)
+    group(g, p.group_starts[g], g < p.NG ? p.group_starts[g + 1] : 0, g < p.NG ? p.prefix_lens[g] : 0);
   fault = __syncthreads_or(bad);
   if (fault) return {0, 0, 4};
   int carry = 0;
@@ -938,12 +945,21 @@ void shared_kernel(const SharedParams p) {
   int fault;
   const ShPlan pl = plan_scan(p, s_tab, reinterpret_cast<int32_t*>(lds), fault);
   const int n = p.NG + p.B;
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == gridDim.x - 1) {  // (the last stretch is the shortest)
     if (threadIdx.x == 0) {
       p.ws_meta[0] = pl.share;
       p.ws_meta[1] = fault;
     }
-    for (int i = threadIdx.x; i <= n; i += kShThreads) p.ws_meta[2 + i] = fault ? 0 : s_tab.cum[i];
+    for (int b = threadIdx.x; b < p.B && !fault; b += kShThreads) {
+      const int g = group_of(s_tab.start, p.NG, b), b0 = g < 0 ? b : s_tab.start[g];
+      int32_t* m = p.ws_meta + kSharedMeta * (b + 1);
+      m[0] = s_tab.pre[b];
+      m[1] = s_tab.ctx[b];
+      m[2] = b0;
+      m[3] = g < 0 ? 0 : (s_tab.start[g + 1] - b0) * p.SG;
+      m[4] = g < 0 ? 0 : s_tab.cum[g];
+      m[5] = s_tab.cum[p.NG + b];
+    }
   }
   if (fault) return;
 

@@ -2,7 +2,7 @@
 // the output rows:
 //   M = max_i m_i, out = sum_i 2^(m_i - M) acc_i / sum_i 2^(m_i - M) l_i
 // over the pieces of the row's prefix unit and of its own keys' unit, whose places
-// follow from the cost sums that the first launch left in the workspace.  One wave
+// follow from the plan that the first launch left in the workspace.  One wave
 // per row, as pa_reduce.hip: lane (r, c) reads dims 4c .. 4c + 3 of every RI-th
 // state, a round of NL loads covers NL * RI of them.
 #include "pa_shared.hpp"
@@ -25,31 +25,26 @@ __global__ __launch_bounds__(64 * kMergeWaves) void shared_merge_kernel(const Sh
   const int b = (int)(row / p.S), s = (int)(row - (int64_t)b * p.S);
   const int kvh = h / p.G;
   const int mine = s * p.G + (h - kvh * p.G);  // row among the sequence's
-  const int32_t* cum = p.ws_meta + 2;
+  const int32_t* meta = p.ws_meta + kSharedMeta * (b + 1);
   const int share = p.ws_meta[0], maxctx = p.MB * p.BS;
-  const int ctx = max(p.context_lens[b], 0);
+  const int P = meta[0], ctx = max(meta[1], 0), b0 = meta[2], rows = meta[3], cum_group = meta[4], cum_own = meta[5];
   const int keys = ctx - p.S + s + 1;  // that the row attends
-  bool bad = p.ws_meta[1] != 0 || ctx > maxctx;
+  const bool bad = p.ws_meta[1] != 0 || ctx > maxctx || (P > maxctx && ctx > 0);
 
   // The states: n1 of the prefix from workspace row a1 on, n2 of the own keys from a2.
   int n1 = 0, n2 = 0, step2 = kSharedWide;
   int64_t a1 = 0, a2 = 0;
   if (!bad && keys > 0) {
-    const int g = group_of(p.group_starts, p.NG, b);
-    const int P = g < 0 ? 0 : prefix_of(p.prefix_lens[g]);
-    bad = P > maxctx;
-    if (!bad && P > 0) {
-      const int b0 = p.group_starts[g], rows = (p.group_starts[g + 1] - b0) * p.SG;
+    int first;
+    if (P > 0) {
       const int at = (b - b0) * p.SG + mine, tiles = wide_tiles(P);
       const int unit = kvh * row_blocks(rows) + at / kSharedWide;
-      int first;
-      unit_workers(cum[g] + unit * wide_cost(tiles), kSharedWideStart, kSharedWideCost, tiles, share, first, n1);
+      unit_workers(cum_group + unit * wide_cost(tiles), kSharedWideStart, kSharedWideCost, tiles, share, first, n1);
       a1 = prefix_slot(p, first, b0, rows, kvh, at);
     }
-    if (!bad && ctx > P) {
+    if (ctx > P) {
       const int tiles = own_tiles(p, ctx - own_first(P));
-      const int unit = kvh * p.own_rb + mine / kSharedWide, begin = cum[p.NG + b] + unit * own_cost(p, tiles);
-      int first;
+      const int begin = cum_own + (kvh * p.own_rb + mine / kSharedWide) * own_cost(p, tiles);
       if (p.thin) {
         unit_workers(begin, kSharedThinStart, kSharedThinCost, tiles, share / kShWaves, first, n2);
         step2 = kSharedThin;
