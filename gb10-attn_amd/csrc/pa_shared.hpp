@@ -793,7 +793,8 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
 #pragma unroll
     for (int i = 0; i < NDMA; ++i) {
       const int row = i * TPD + lane / NCH;
-      tv[i] = *reinterpret_cast<const typename Tl::Raw*>(vbase + shfl64(r.v, row) + (lane % NCH) * 8 * EB);
+      // (Streamed: read once.  32/8 heads of 128, 4 x 32 sequences: 93 -> 88 us.)
+      tv[i] = load_raw<KV>(vbase, (int64_t)(shfl64(r.v, row) + (lane % NCH) * 8 * EB));
     }
   };
   int32_t blk = page_at(0);

@@ -56,30 +56,37 @@ __global__ __launch_bounds__(64 * kMergeWaves) void shared_merge_kernel(const Sh
   }
   auto place = [&](int i) { return i < n1 ? a1 + (int64_t)i * kSharedWide : a2 + (int64_t)(i - n1) * step2; };
   const int all = n1 + n2;
-  float M = -__builtin_inff();
-  for (int i0 = 0; i0 < all; i0 += 64)
-    M = fmaxf(M, i0 + lane < all ? p.ws_m[place(i0 + lane)] : -__builtin_inff());
+  // One round trip: the first 64 states' maxima and sums, and the first round of rows.
+  float4_t x[NL];
+  auto load_rows = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = i0 + j * RI + r;
+      x[j] = i < all ? *reinterpret_cast<const float4_t*>(p.ws_acc + place(i) * D + 4 * c) : float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  float m = -__builtin_inff(), l = 0.0f;
+  auto load_states = [&](int i0) {
+    const bool on = i0 + lane < all;
+    const int64_t at = place(on ? i0 + lane : 0);
+    m = on ? p.ws_m[at] : -__builtin_inff();
+    l = on ? p.ws_l[at] : 0.0f;
+  };
+  load_states(0);
+  load_rows(0);
+  float M = m;
+  for (int i0 = 64; i0 < all; i0 += 64) M = fmaxf(M, i0 + lane < all ? p.ws_m[place(i0 + lane)] : -__builtin_inff());
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   float4_t acc = float4_t{0.f, 0.f, 0.f, 0.f};
   float L = 0.0f;
   for (int i0 = 0; i0 < all; i0 += 64) {
-    float w = 0.0f;
-    if (i0 + lane < all) {
-      const int64_t at = place(i0 + lane);
-      const float m = p.ws_m[at], l = p.ws_l[at];
-      // (A state that saw no key, or a key that cannot be read, has m = -inf: l says which.)
-      w = m == -__builtin_inff() ? 0.0f : fast_exp2(m - M);
-      L += l != l ? l : w * l;
-    }
+    if (i0 > 0) load_states(i0);
+    // (A state that saw no key, or a key that cannot be read, has m = -inf: l says which.)
+    const float w = m == -__builtin_inff() ? 0.0f : fast_exp2(m - M);
+    L += l != l ? l : w * l;
     for (int k = 0; k < 64 && i0 + k < all; k += NL * RI) {
-      float4_t x[NL];
-#pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const int i = k + j * RI + r;
-        x[j] = i < 64 && i0 + i < all ? *reinterpret_cast<const float4_t*>(p.ws_acc + place(i0 + i) * D + 4 * c)
-                                      : float4_t{0.f, 0.f, 0.f, 0.f};
-      }
+      if (i0 + k > 0) load_rows(i0 + k);
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const float wi = __shfl(w, (k + j * RI + r) & 63, 64);
