@@ -1369,6 +1369,9 @@ extern "C" int pa_qk_norm_rope_write_kv(pa_tensor_t* q_out, pa_tensor_t* k_cache
   auto in_range = [](float r) { return std::fabs(r) >= 0x1p-60f && std::fabs(r) <= 0x1p60f; };
   p.k_fast = in_range(p.k_rcp); p.v_fast = in_range(p.v_rcp);
   p.unit_scale = p.k_scale == 1.0f && p.v_scale == 1.0f;
+  // (1 / s exact: s is a power of two whose inverse is normal too.)
+  auto power = [&](float s) { int e; return in_range(s) && std::fabs(std::frexp(s, &e)) == 0.5f; };
+  p.k_exact = power(p.k_scale); p.v_exact = power(p.v_scale);
   p.eps = (float)eps; p.inv_d = 1.0f / (float)D;
   p.bs_div = make_fastdiv((uint32_t)BS);
   return hip_status(launch_qk_norm_rope(p, static_cast<hipStream_t>(stream)), "norm and rotation kernel launch");

@@ -235,9 +235,11 @@ struct RopeParams {
   int32_t T, H, HKV, D, BS, rot, interleaved;
   int32_t act_dtype, cache_dtype, out_dtype, weight_dtype, table_dtype, slot_i64, pos_i64;
   int32_t unit_scale, k_fast, v_fast;  // as WriteParams
+  int32_t k_exact, v_exact;            // k_scale / v_scale is a power of two: multiply by its inverse
+  int32_t q_blocks, kv_blocks;         // work-groups of the query heads, and of the keys' or the values'
   float k_scale, v_scale, k_rcp, v_rcp;
   float eps, inv_d;
-  FastDiv bs_div, slice_div;
+  FastDiv bs_div, q_slices, kv_slices;
 };
 
 // Pages of the cache moved, forked and compacted.  A cache is [L, NB, BS, row]

@@ -16,7 +16,7 @@
 // of its pairs are its own (chunks u and u + rot / 16; interleaved pairs are
 // neighbours): the rotation needs no exchange, the norm one sum over the D / 16
 // lanes of a row.  A lane group takes kRows heads of one token, all loaded
-// before the first is used, with the same eight cosines and sines.
+// before the first is used, with the same eight cosines, sines and weights.
 #include "pa_convert.hpp"
 
 #include <algorithm>
@@ -37,18 +37,32 @@ __device__ inline int64_t load_index(const void* p, int i64, int64_t i) {
   return i64 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
 }
 
-// LPR: lanes per row (a power of two, D / 16 of them in use).
-template <int ACT, int DST, int LPR, int kRows>
-__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(const RopeParams p) {
-  const uint32_t idx = blockIdx.x * kRopeThreads + threadIdx.x;
+enum RopeKind { kRopeQ, kRopeK, kRopeV };
+
+// x / s rounded to nearest: fast as div_rn; exact: 1 / s is a power of two.
+__device__ inline void divide8(float (&x)[8], float s, float r, bool exact, bool fast) {
+  if (exact) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= r;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = div_rn(x[e], s, r, fast);
+  }
+}
+
+// One work-group's share of the query, key or value heads: a group of LPR lanes (a
+// power of two, D / 16 of them in use) takes kRows heads of one token.  idx: the
+// thread among those of its kind.
+template <int ACT, int DST, int LPR, int kRows, int kKind>
+__device__ __forceinline__ void rope_heads(const RopeParams& p, uint32_t idx, const FastDiv& slices, int heads) {
   const uint32_t grp = idx / LPR;
-  const uint32_t tl = fastdiv(grp, p.slice_div);  // token of this launch
+  const uint32_t tl = fastdiv(grp, slices);  // token of this launch
   if (tl >= (uint32_t)p.T) return;
-  const int head0 = (int)(grp - tl * p.slice_div.d) * kRows;
+  const int head0 = (int)(grp - tl * slices.d) * kRows;
   const int64_t t = p.t_base + tl;
   const int u = (int)(idx % LPR);
   const bool on = u < p.D / 16;
-  const bool turned = u < p.rot / 16;
+  const bool turned = kKind != kRopeV && u < p.rot / 16;
   int a0, a1;  // first elements of this lane's chunks
   if (p.interleaved || !turned) {
     a0 = 16 * u;
@@ -57,74 +71,68 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(const RopePa
     a0 = 8 * u;
     a1 = p.rot / 2 + 8 * u;
   }
-  const int heads = p.H + 2 * p.HKV;
+  const void* src = kKind == kRopeQ ? p.q : kKind == kRopeK ? p.key : p.value;
+  const int64_t sh = kKind == kRopeQ ? p.q_sh : kKind == kRopeK ? p.key_sh : p.val_sh;
+  const int64_t st = kKind == kRopeQ ? p.q_st : kKind == kRopeK ? p.key_st : p.val_st;
 
   float x[kRows][16];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int h = head0 + r;
-    const void* src = nullptr;
-    int64_t off = 0;
-    if (h < p.H) {
-      src = p.q;
-      off = t * p.q_st + (int64_t)h * p.q_sh;
-    } else if (h < p.H + p.HKV) {
-      src = p.key;
-      off = t * p.key_st + (int64_t)(h - p.H) * p.key_sh;
-    } else {
-      src = p.value;
-      off = t * p.val_st + (int64_t)(h - p.H - p.HKV) * p.val_sh;
-    }
-    if (on && h < heads) {
-      float c[8], d[8];
+    float c[8], d[8];
+    if (on && head0 + r < heads) {
+      const int64_t off = t * st + (int64_t)(head0 + r) * sh;
       load8<ACT>(src, off + a0, c);
       load8<ACT>(src, off + a1, d);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[r][e] = c[e];
-        x[r][8 + e] = d[e];
+      for (int e = 0; e < 8; ++e) c[e] = d[e] = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[r][e] = c[e];
+      x[r][8 + e] = d[e];
+    }
+  }
+  int64_t slot = 0;
+  if constexpr (kKind != kRopeQ) slot = load_index(p.slots, p.slot_i64, t);
+  float cs[8], sn[8], w0[8], w1[8];
+  const void* w = kKind == kRopeQ ? p.q_weight : p.k_weight;
+  if constexpr (kKind != kRopeV) {
+    if (turned) {
+      const int64_t pos = load_index(p.positions, p.pos_i64, t);
+      if (pos >= 0 && pos < p.table_rows) {
+        load8_any(p.table, p.table_dtype, pos * p.table_st + 8 * u, cs);
+        load8_any(p.table, p.table_dtype, pos * p.table_st + p.rot / 2 + 8 * u, sn);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cs[e] = sn[e] = __builtin_nanf("");
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[r][e] = 0.0f;
+    }
+    if (w && on) {
+      load8_any(w, p.weight_dtype, a0, w0);
+      load8_any(w, p.weight_dtype, a1, w1);
     }
   }
-
-  float cs[8], sn[8];
-  if (turned && head0 < p.H + p.HKV) {
-    const int64_t pos = load_index(p.positions, p.pos_i64, t);
-    if (pos >= 0 && pos < p.table_rows) {
-      load8_any(p.table, p.table_dtype, pos * p.table_st + 8 * u, cs);
-      load8_any(p.table, p.table_dtype, pos * p.table_st + p.rot / 2 + 8 * u, sn);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) cs[e] = sn[e] = __builtin_nanf("");
-    }
-  }
-  const int64_t slot = head0 + kRows > p.H ? load_index(p.slots, p.slot_i64, t) : -1;
 
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int h = head0 + r;
-    const bool is_q = h < p.H, is_v = h >= p.H + p.HKV;
-    const void* w = is_q ? p.q_weight : p.k_weight;
-    float ss = 0.0f;
+    if constexpr (kKind != kRopeV) {
+      if (w) {  // (the same for every lane)
+        float ss = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) ss = fmaf(x[r][e], x[r][e], ss);
-    ss = group_sum<LPR>(ss);  // (every lane of the group takes part)
-    if (!on || h >= heads) continue;
-    if (!is_v) {
-      if (w) {
+        for (int e = 0; e < 16; ++e) ss = fmaf(x[r][e], x[r][e], ss);
+        ss = group_sum<LPR>(ss);  // (every lane of the group takes part)
         const float rms = 1.0f / __builtin_sqrtf(fmaf(ss, p.inv_d, p.eps));
-        float w0[8], w1[8];
-        load8_any(w, p.weight_dtype, a0, w0);
-        load8_any(w, p.weight_dtype, a1, w1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[r][e] = x[r][e] * rms * w0[e];
-          x[r][8 + e] = x[r][8 + e] * rms * w1[e];
+          x[r][e] *= rms * w0[e];
+          x[r][8 + e] *= rms * w1[e];
         }
       }
+    }
+    if (!on || h >= heads) continue;
+    if constexpr (kKind != kRopeV) {
       if (turned) {
         if (p.interleaved) {
 #pragma unroll
@@ -149,52 +157,67 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(const RopePa
       lo[e] = x[r][e];
       hi[e] = x[r][8 + e];
     }
-    if (is_q) {
+    if constexpr (kKind == kRopeQ) {
       const int64_t o = t * p.out_st + (int64_t)h * p.out_sh;
       switch (p.out_dtype) {
         case kF16: store8<kF16>(p.q_out, o + a0, lo); store8<kF16>(p.q_out, o + a1, hi); break;
         case kBF16: store8<kBF16>(p.q_out, o + a0, lo); store8<kBF16>(p.q_out, o + a1, hi); break;
         default: store8<kF32>(p.q_out, o + a0, lo); store8<kF32>(p.q_out, o + a1, hi); break;
       }
-      continue;
-    }
-    if (slot < 0 || slot >= p.nslots) continue;
-    const uint32_t blk = fastdiv((uint32_t)slot, p.bs_div);
-    const uint32_t row = (uint32_t)slot - blk * (uint32_t)p.BS;
-    if (!p.unit_scale) {
-      const float s = is_v ? p.v_scale : p.k_scale, rc = is_v ? p.v_rcp : p.k_rcp;
-      const bool fast = is_v ? p.v_fast : p.k_fast;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo[e] = div_rn(lo[e], s, rc, fast);
-        hi[e] = div_rn(hi[e], s, rc, fast);
+    } else {
+      if (slot < 0 || slot >= p.nslots) continue;
+      const uint32_t blk = fastdiv((uint32_t)slot, p.bs_div);
+      const uint32_t row = (uint32_t)slot - blk * (uint32_t)p.BS;
+      if (!p.unit_scale) {
+        const float s = kKind == kRopeV ? p.v_scale : p.k_scale, rc = kKind == kRopeV ? p.v_rcp : p.k_rcp;
+        const bool fast = kKind == kRopeV ? p.v_fast : p.k_fast, exact = kKind == kRopeV ? p.v_exact : p.k_exact;
+        divide8(lo, s, rc, exact, fast);
+        divide8(hi, s, rc, exact, fast);
       }
+      void* c = kKind == kRopeV ? p.vc : p.kc;
+      const int64_t d = kKind == kRopeV ? (int64_t)blk * p.vc_sb + (int64_t)row * p.vc_st + (int64_t)h * p.vc_sh
+                                        : (int64_t)blk * p.kc_sb + (int64_t)row * p.kc_st + (int64_t)h * p.kc_sh;
+      store8<DST>(c, d + a0, lo);
+      store8<DST>(c, d + a1, hi);
     }
-    const int hk = is_v ? h - p.H - p.HKV : h - p.H;
-    const int64_t d = is_v ? (int64_t)blk * p.vc_sb + (int64_t)row * p.vc_st + (int64_t)hk * p.vc_sh
-                           : (int64_t)blk * p.kc_sb + (int64_t)row * p.kc_st + (int64_t)hk * p.kc_sh;
-    void* c = is_v ? p.vc : p.kc;
-    store8<DST>(c, d + a0, lo);
-    store8<DST>(c, d + a1, hi);
   }
 }
 
-// Lane groups per launch: fewer than 2^27, so that thread indices stay below 2^31.
+// Query heads' work-groups first, then keys', then values': a wave serves one kind
+// (with the kinds mixed in a wave it ran every kind's code: 8192 tokens of 32/8
+// heads of 128 into FP8 63 us, so 43).
+template <int ACT, int DST, int LPR, int kRows>
+__global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(const RopeParams p) {
+  int b = blockIdx.x;
+  if (b < p.q_blocks) {
+    rope_heads<ACT, DST, LPR, kRows, kRopeQ>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.q_slices, p.H);
+  } else if ((b -= p.q_blocks) < p.kv_blocks) {
+    rope_heads<ACT, DST, LPR, kRows, kRopeK>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_slices, p.HKV);
+  } else {
+    b -= p.kv_blocks;
+    rope_heads<ACT, DST, LPR, kRows, kRopeV>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_slices, p.HKV);
+  }
+}
+
+// Lane groups per launch and kind: fewer than 2^27, so that thread indices stay below 2^31.
 constexpr int64_t kRopeMaxGroups = (int64_t)1 << 26;
 
 template <int ACT, int DST, int LPR, int kRows>
 static hipError_t launch_r(const RopeParams& p0, hipStream_t stream) {
   RopeParams p = p0;
-  const int64_t slices = (p.H + 2 * (int64_t)p.HKV + kRows - 1) / kRows;
-  p.slice_div = make_fastdiv((uint32_t)slices);
-  const int64_t step = std::max<int64_t>(1, kRopeMaxGroups / slices);
+  const int64_t qs = (p.H + kRows - 1) / kRows, ks = (p.HKV + kRows - 1) / kRows;
+  p.q_slices = make_fastdiv((uint32_t)std::max<int64_t>(1, qs));
+  p.kv_slices = make_fastdiv((uint32_t)std::max<int64_t>(1, ks));
+  const int64_t step = std::max<int64_t>(1, kRopeMaxGroups / std::max<int64_t>(1, std::max(qs, ks)));
   note_launch("pa::qk_norm_rope_kernel<%d, %d, %d, %d>", ACT, DST, LPR, kRows);
   for (int64_t t = 0; t < p0.T; t += step) {
     p.t_base = t;
     p.T = (int32_t)std::min<int64_t>(step, p0.T - t);
-    const int64_t threads = p.T * slices * LPR;
-    hipLaunchKernelGGL((qk_norm_rope_kernel<ACT, DST, LPR, kRows>),
-                       dim3((unsigned)((threads + kRopeThreads - 1) / kRopeThreads)), dim3(kRopeThreads), 0, stream, p);
+    auto blocks = [&](int64_t slices) { return (int32_t)((p.T * slices * LPR + kRopeThreads - 1) / kRopeThreads); };
+    p.q_blocks = blocks(qs);
+    p.kv_blocks = blocks(ks);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<ACT, DST, LPR, kRows>), dim3((unsigned)(p.q_blocks + 2 * p.kv_blocks)),
+                       dim3(kRopeThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

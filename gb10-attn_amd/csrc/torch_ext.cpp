@@ -284,21 +284,56 @@ void one_device(const at::Tensor& q, std::initializer_list<const at::Tensor*> ot
     TORCH_CHECK(t->device() == q.device(), "all tensors must be on one device");
 }
 
-void op_qk_norm_rope_write_kv_out(const at::Tensor& q, const at::Tensor& key, const at::Tensor& value,
-                                  const at::Tensor& k_cache, const at::Tensor& v_cache,
-                                  const at::Tensor& slot_mapping, const at::Tensor& cos_sin,
-                                  const at::Tensor& positions, const std::optional<at::Tensor>& q_weight,
-                                  const std::optional<at::Tensor>& k_weight, double eps, bool interleaved,
-                                  double k_scale, double v_scale, const at::Tensor& out) {
-  one_device(q, {&key, &value, &k_cache, &v_cache, &slot_mapping, &cos_sin, &positions, &out});
-  for (const auto* w : {&q_weight, &k_weight})
+// t, or a copy where the row kernels cannot read it in place (last dimension,
+// alignment, negative strides).
+at::Tensor rows_of(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    ok = ok && t.stride(i) >= 0 && ((t.stride(i) * t.element_size()) % 16 == 0 || t.size(i) == 1);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+std::optional<at::Tensor> rows_of(const std::optional<at::Tensor>& t) {
+  return t.has_value() ? std::optional<at::Tensor>(rows_of(*t)) : t;
+}
+
+// Integer vectors as the entry points take them: int32 or int64 (int32 alone with
+// `narrow`), contiguous, on the device.
+at::Tensor index_of(const at::Tensor& t, const at::Device& dev, bool narrow) {
+  const at::ScalarType ty = t.scalar_type();
+  const at::ScalarType want = narrow ? at::kInt : ty == at::kInt || ty == at::kLong ? ty : at::kLong;
+  return t.to(dev, want).contiguous();
+}
+
+at::Tensor op_qk_norm_rope_write_kv(const at::Tensor& q0, const at::Tensor& key0, const at::Tensor& value0,
+                                    const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                    const at::Tensor& slot_mapping, const at::Tensor& cos_sin,
+                                    const at::Tensor& positions, const std::optional<at::Tensor>& q_weight,
+                                    const std::optional<at::Tensor>& k_weight, double eps, bool interleaved,
+                                    double k_scale, double v_scale, std::optional<at::ScalarType> out_dtype,
+                                    const std::optional<at::Tensor>& out) {
+  TORCH_CHECK(q0.is_cuda(), "q must be on CUDA");
+  TORCH_CHECK(key0.is_cuda(), "key must be on CUDA");
+  TORCH_CHECK(value0.is_cuda(), "value must be on CUDA");
+  TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda(), "k_cache and v_cache must be on CUDA");
+  TORCH_CHECK(q0.dim() == 3 && key0.dim() == 3 && value0.dim() == 3, "q must be [T, H, D], key/value [T, HKV, D]");
+  TORCH_CHECK(kv_addressable(k_cache) && kv_addressable(v_cache),
+              "k_cache/v_cache must be 16-byte aligned [NB, BS, HKV, D] views with a contiguous last dim");
+  c10::DeviceGuard guard(q0.device());
+  const at::Tensor q = rows_of(q0), key = rows_of(key0), value = rows_of(value0), table = rows_of(cos_sin);
+  const auto qw = rows_of(q_weight), kw = rows_of(k_weight);
+  const at::Tensor slots = index_of(slot_mapping, q.device(), false), pos = index_of(positions, q.device(), false);
+  const at::Tensor o =
+      out.has_value() ? *out : at::empty(q.sizes(), q.options().dtype(out_dtype.value_or(q.scalar_type())));
+  one_device(q, {&key, &value, &k_cache, &v_cache, &table, &o});
+  for (const auto* w : {&qw, &kw})
     if (w->has_value()) one_device(q, {&**w});
-  c10::DeviceGuard guard(q.device());
-  pa_tensor_t o = view(out), kc = view(k_cache), vc = view(v_cache), qq = view(q), kk = view(key), vv = view(value),
-              ss = view(slot_mapping), cs = view(cos_sin), pp = view(positions);
-  OptView qw(q_weight), kw(k_weight);
-  check(pa_qk_norm_rope_write_kv(&o, &kc, &vc, &qq, &kk, &vv, &ss, &cs, &pp, qw.get(), kw.get(), eps,
+  pa_tensor_t oo = view(o), kc = view(k_cache), vc = view(v_cache), qq = view(q), kk = view(key), vv = view(value),
+              ss = view(slots), cs = view(table), pp = view(pos);
+  OptView qv(qw), kv(kw);
+  check(pa_qk_norm_rope_write_kv(&oo, &kc, &vc, &qq, &kk, &vv, &ss, &cs, &pp, qv.get(), kv.get(), eps,
                                  interleaved ? 1 : 0, k_scale, v_scale, stream_of(q)));
+  return o;
 }
 
 void op_shared_prefix_out(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt,
@@ -316,51 +351,92 @@ void op_shared_prefix_out(const at::Tensor& q, const at::Tensor& k, const at::Te
                                       stream_of(a.q)));
 }
 
+// A cache [NB, BS, HKV, D] or [L, NB, BS, HKV, D] as [L, NB, BS, HKV * D].
+struct Pages {
+  pa_tensor_t t;
+  bool have = false;
+  explicit Pages(const std::optional<at::Tensor>& x) {
+    if (x.has_value()) *this = Pages(*x);
+  }
+  explicit Pages(const at::Tensor& x) : have(true) {
+    TORCH_CHECK(x.is_cuda(), "kv cache must be on CUDA");
+    TORCH_CHECK(x.dim() == 4 || x.dim() == 5, "k_cache/v_cache must be [NB, BS, HKV, D] or [L, NB, BS, HKV, D]");
+    const int64_t d = x.dim() - 4, H = x.size(-2), D = x.size(-1);
+    TORCH_CHECK((D <= 1 || x.stride(-1) == 1) && (H <= 1 || x.stride(-2) == D),
+                "k_cache/v_cache must have contiguous token rows");
+    std::memset(&t, 0, sizeof(t));
+    t.data = x.data_ptr();
+    t.dtype = pa_dtype(x.scalar_type());
+    t.ndim = 4;
+    t.shape[0] = d ? x.size(0) : 1;
+    t.stride[0] = d ? x.stride(0) : 0;
+    for (int i = 0; i < 2; ++i) {
+      t.shape[1 + i] = x.size(d + i);
+      t.stride[1 + i] = x.stride(d + i);
+    }
+    t.shape[3] = H * D;
+    t.stride[3] = 1;
+  }
+  pa_tensor_t* get() { return have ? &t : nullptr; }
+};
+
+// Tables, lengths and counts are updated in place.
+void state(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->is_cuda(),
+                "block_tables, context_lens and page_refs must be int32 on CUDA");
+}
+
 void op_copy_pages(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache, const at::Tensor& src,
                    const at::Tensor& dst) {
-  one_device(k_cache, {&src, &dst});
-  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  Pages k(k_cache), v(v_cache);
+  if (v.have) one_device(k_cache, {&*v_cache});
   c10::DeviceGuard guard(k_cache.device());
-  pa_tensor_t k = view(k_cache), s = view(src), d = view(dst);
-  OptView v(v_cache);
-  check(pa_copy_pages(&k, v.get(), &s, &d, stream_of(k_cache)));
+  const at::Tensor a = index_of(src, k_cache.device(), true), b = index_of(dst, k_cache.device(), true);
+  pa_tensor_t s = view(a), d = view(b);
+  check(pa_copy_pages(k.get(), v.get(), &s, &d, stream_of(k_cache)));
 }
 
 at::Tensor op_fork_sequences(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache,
                              const at::Tensor& block_tables, const at::Tensor& context_lens,
                              const at::Tensor& page_refs, const at::Tensor& parents, const at::Tensor& rows) {
-  one_device(k_cache, {&block_tables, &context_lens, &page_refs, &parents, &rows});
-  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  state({&block_tables, &context_lens, &page_refs});
+  Pages k(k_cache), v(v_cache);
+  one_device(k_cache, {&block_tables, &context_lens, &page_refs});
+  if (v.have) one_device(k_cache, {&*v_cache});
   c10::DeviceGuard guard(k_cache.device());
-  at::Tensor copied = at::empty(rows.sizes(), rows.options());
-  pa_tensor_t k = view(k_cache), bt = view(block_tables), cl = view(context_lens), rf = view(page_refs),
-              pr = view(parents), rw = view(rows), cp = view(copied);
-  OptView v(v_cache);
+  const at::Tensor from = index_of(parents, k_cache.device(), true), to = index_of(rows, k_cache.device(), true);
+  at::Tensor copied = at::empty(to.sizes(), to.options());
+  pa_tensor_t bt = view(block_tables), cl = view(context_lens), rf = view(page_refs), pr = view(from), rw = view(to),
+              cp = view(copied);
   Scratch s = scratch_of(k_cache, pa_fork_workspace_size(&bt, &rf, &rw));
-  check(pa_fork_sequences(&k, v.get(), &bt, &cl, &rf, &pr, &rw, &cp, s.ptr, s.bytes, stream_of(k_cache)));
+  check(pa_fork_sequences(k.get(), v.get(), &bt, &cl, &rf, &pr, &rw, &cp, s.ptr, s.bytes, stream_of(k_cache)));
   return copied;
 }
 
 void op_free_sequences(const at::Tensor& block_tables, const at::Tensor& context_lens, const at::Tensor& page_refs,
                        const at::Tensor& rows, int64_t block_size) {
-  one_device(block_tables, {&context_lens, &page_refs, &rows});
+  state({&block_tables, &context_lens, &page_refs});
+  one_device(block_tables, {&context_lens, &page_refs});
   c10::DeviceGuard guard(block_tables.device());
-  pa_tensor_t bt = view(block_tables), cl = view(context_lens), rf = view(page_refs), rw = view(rows);
+  const at::Tensor to = index_of(rows, block_tables.device(), true);
+  pa_tensor_t bt = view(block_tables), cl = view(context_lens), rf = view(page_refs), rw = view(to);
   check(pa_free_sequences(&bt, &cl, &rf, &rw, block_size, stream_of(block_tables)));
 }
 
 std::tuple<at::Tensor, at::Tensor> op_compact_pages(const at::Tensor& k_cache, const std::optional<at::Tensor>& v_cache,
                                                     const at::Tensor& block_tables, const at::Tensor& page_refs,
                                                     const at::Tensor& tables_out, const at::Tensor& refs_out) {
+  state({&block_tables, &page_refs, &tables_out, &refs_out});
+  Pages k(k_cache), v(v_cache);
   one_device(k_cache, {&block_tables, &page_refs, &tables_out, &refs_out});
-  if (v_cache.has_value()) one_device(k_cache, {&*v_cache});
+  if (v.have) one_device(k_cache, {&*v_cache});
   c10::DeviceGuard guard(k_cache.device());
   at::Tensor map = at::empty(page_refs.sizes(), page_refs.options()), n = at::empty({1}, page_refs.options());
-  pa_tensor_t k = view(k_cache), bt = view(block_tables), rf = view(page_refs), to = view(tables_out),
-              ro = view(refs_out), mp = view(map), nl = view(n);
-  OptView v(v_cache);
+  pa_tensor_t bt = view(block_tables), rf = view(page_refs), to = view(tables_out), ro = view(refs_out),
+              mp = view(map), nl = view(n);
   Scratch s = scratch_of(k_cache, pa_compact_workspace_size(&rf));
-  check(pa_compact_pages(&k, v.get(), &bt, &rf, &to, &ro, &mp, &nl, s.ptr, s.bytes, stream_of(k_cache)));
+  check(pa_compact_pages(k.get(), v.get(), &bt, &rf, &to, &ro, &mp, &nl, s.ptr, s.bytes, stream_of(k_cache)));
   return {map, n};
 }
 
@@ -402,9 +478,9 @@ TORCH_LIBRARY(gb10_attn, m) {
   m.def("write_kv_scaled(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor key, Tensor value, Tensor slot_mapping, "
         "float k_scale, float v_scale) -> ()",
         &op_write_kv_scaled);
-  m.def("qk_norm_rope_write_kv_out(Tensor q, Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+  m.def("qk_norm_rope_write_kv(Tensor q, Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, "
         "Tensor slot_mapping, Tensor cos_sin, Tensor positions, Tensor? q_weight, Tensor? k_weight, float eps, "
-        "bool interleaved, float k_scale, float v_scale, Tensor(c!) out) -> ()");
+        "bool interleaved, float k_scale, float v_scale, ScalarType? out_dtype, Tensor? out) -> Tensor");
   m.def("shared_prefix_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor context_lens, "
         "Tensor group_starts, Tensor prefix_lens, float scale, float k_scale, float v_scale, Tensor(a!) out) -> ()");
   m.def("copy_pages(Tensor(a!) k_cache, Tensor(b!)? v_cache, Tensor src, Tensor dst) -> ()");
@@ -422,7 +498,7 @@ TORCH_LIBRARY_IMPL(gb10_attn, CUDA, m) {
   m.impl("decode_out", &op_decode_out);
   m.impl("prefill_out", &op_prefill_out);
   m.impl("write_kv_into", &op_write_kv_into);
-  m.impl("qk_norm_rope_write_kv_out", &op_qk_norm_rope_write_kv_out);
+  m.impl("qk_norm_rope_write_kv", &op_qk_norm_rope_write_kv);
   m.impl("shared_prefix_out", &op_shared_prefix_out);
   m.impl("copy_pages", &op_copy_pages);
   m.impl("fork_sequences", &op_fork_sequences);

@@ -128,12 +128,24 @@ class _CAbi:
                                            k_scale, v_scale, _stream(key.device)))
 
     @staticmethod
-    def qk_norm_rope_write_kv_out(q, key, value, k_cache, v_cache, slot_mapping, cos_sin, positions, q_weight, k_weight,
-                                  eps, interleaved, k_scale, v_scale, out):
+    def qk_norm_rope_write_kv(q, key, value, k_cache, v_cache, slot_mapping, cos_sin, positions, q_weight, k_weight,
+                              eps, interleaved, k_scale, v_scale, out_dtype, out):
+        for t, n in ((q, "q"), (key, "key"), (value, "value"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+            if not t.is_cuda:
+                raise RuntimeError(f"{n} must be on CUDA")
+        if q.dim() != 3 or key.dim() != 3 or value.dim() != 3:
+            raise RuntimeError("q must be [T, H, D], key/value [T, HKV, D]")
+        if not _kv_ok(k_cache) or not _kv_ok(v_cache):
+            raise RuntimeError("k_cache/v_cache must be 16-byte aligned [NB, BS, HKV, D] views with a contiguous last dim")
+        o = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device) if out is None else out
+        q, key, value, cos_sin = (_rows(t) for t in (q, key, value, cos_sin))
+        q_weight, k_weight = (t if t is None else _rows(t) for t in (q_weight, k_weight))
+        slot_mapping, positions = (_index(t, q.device) for t in (slot_mapping, positions))
         with torch.cuda.device(q.device):
-            check(lib().pa_qk_norm_rope_write_kv(*_refs(out, k_cache, v_cache, q, key, value, slot_mapping, cos_sin,
+            check(lib().pa_qk_norm_rope_write_kv(*_refs(o, k_cache, v_cache, q, key, value, slot_mapping, cos_sin,
                                                         positions, q_weight, k_weight), eps, int(interleaved), k_scale,
                                                  v_scale, _stream(q.device)))
+        return o
 
     @staticmethod
     def shared_prefix_out(q, k_cache, v_cache, block_tables, context_lens, group_starts, prefix_lens, scale, k_scale,
@@ -150,32 +162,40 @@ class _CAbi:
 
     @staticmethod
     def copy_pages(k_cache, v_cache, src, dst):
-        with torch.cuda.device(k_cache.device):
-            check(lib().pa_copy_pages(*_refs(k_cache, v_cache, src, dst), _stream(k_cache.device)))
+        k = _pages(k_cache)
+        src, dst = (t.to(k.device, torch.int32).contiguous() for t in (src, dst))
+        with torch.cuda.device(k.device):
+            check(lib().pa_copy_pages(*_refs(k, _pages(v_cache), src, dst), _stream(k.device)))
 
     @staticmethod
     def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows):
-        copied = torch.empty(rows.shape, dtype=torch.int32, device=rows.device)
-        with torch.cuda.device(rows.device):
-            ws = _scratch(lib().pa_fork_workspace_size(*_refs(block_tables, page_refs, rows)), rows.device)
-            check(lib().pa_fork_sequences(*_refs(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows,
-                                                 copied), ws.data_ptr(), ws.numel(), _stream(rows.device)))
+        _state(block_tables, context_lens, page_refs)
+        dev = block_tables.device
+        parents, rows = (t.to(dev, torch.int32).contiguous() for t in (parents, rows))
+        copied = torch.empty(rows.shape, dtype=torch.int32, device=dev)
+        with torch.cuda.device(dev):
+            ws = _scratch(lib().pa_fork_workspace_size(*_refs(block_tables, page_refs, rows)), dev)
+            check(lib().pa_fork_sequences(*_refs(_pages(k_cache), _pages(v_cache), block_tables, context_lens, page_refs,
+                                                 parents, rows, copied), ws.data_ptr(), ws.numel(), _stream(dev)))
         return copied
 
     @staticmethod
     def free_sequences(block_tables, context_lens, page_refs, rows, block_size):
-        with torch.cuda.device(rows.device):
-            check(lib().pa_free_sequences(*_refs(block_tables, context_lens, page_refs, rows), block_size,
-                                          _stream(rows.device)))
+        _state(block_tables, context_lens, page_refs)
+        dev = block_tables.device
+        rows = rows.to(dev, torch.int32).contiguous()
+        with torch.cuda.device(dev):
+            check(lib().pa_free_sequences(*_refs(block_tables, context_lens, page_refs, rows), block_size, _stream(dev)))
 
     @staticmethod
     def compact_pages(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out):
+        _state(block_tables, page_refs, tables_out, refs_out)
         dev = page_refs.device
         page_map, n = torch.empty_like(page_refs), torch.empty(1, dtype=torch.int32, device=dev)
         with torch.cuda.device(dev):
             ws = _scratch(lib().pa_compact_workspace_size(*_refs(page_refs)), dev)
-            check(lib().pa_compact_pages(*_refs(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out,
-                                                page_map, n), ws.data_ptr(), ws.numel(), _stream(dev)))
+            check(lib().pa_compact_pages(*_refs(_pages(k_cache), _pages(v_cache), block_tables, page_refs, tables_out,
+                                                refs_out, page_map, n), ws.data_ptr(), ws.numel(), _stream(dev)))
         return page_map, n
 
 
@@ -363,20 +383,8 @@ def qk_norm_rope_write_kv(q, key, value, k_cache, v_cache, slot_mapping, cos_sin
     interleaved=True.  Keys and values go to k_cache/v_cache at slot_mapping as
     write_kv writes them; returns the queries (a new tensor of q's type, out_dtype,
     or `out`, which may be q)."""
-    for t, n in ((q, "q"), (key, "key"), (value, "value"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not t.is_cuda:
-            raise RuntimeError(f"{n} must be on CUDA")
-    if q.dim() != 3 or key.dim() != 3 or value.dim() != 3:
-        raise RuntimeError("q must be [T, H, D], key/value [T, HKV, D]")
-    if not _kv_ok(k_cache) or not _kv_ok(v_cache):
-        raise RuntimeError("k_cache/v_cache must be 16-byte aligned [NB, BS, HKV, D] views with a contiguous last dim")
-    o = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device) if out is None else out
-    q, key, value, cos_sin = (_rows(t) for t in (q, key, value, cos_sin))
-    q_weight, k_weight = (t if t is None else _rows(t) for t in (q_weight, k_weight))
-    _native().qk_norm_rope_write_kv_out(q, key, value, k_cache, v_cache, _index(slot_mapping, q.device), cos_sin,
-                                        _index(positions, q.device), q_weight, k_weight, float(eps), bool(interleaved),
-                                        float(k_scale), float(v_scale), o)
-    return o
+    return _native().qk_norm_rope_write_kv(q, key, value, k_cache, v_cache, slot_mapping, cos_sin, positions, q_weight,
+                                           k_weight, eps, interleaved, k_scale, v_scale, out_dtype, out)
 
 
 def _rows(t):
@@ -420,8 +428,7 @@ def copy_pages(k_cache, v_cache, src, dst):
     """Pages src[i] -> dst[i] of a cache ([NB, BS, HKV, D], or [L, NB, BS, HKV, D] for every layer at once;
     v_cache may be None) in one launch.  Negative or outside pages are skipped; a destination named
     twice takes the last pair that names it (pa_copy_pages).  In place; returns nothing."""
-    k = _pages(k_cache)
-    _native().copy_pages(k, _pages(v_cache), *(t.to(k.device, torch.int32).contiguous() for t in (src, dst)))
+    _native().copy_pages(k_cache, v_cache, src, dst)
 
 
 def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows):
@@ -432,17 +439,12 @@ def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, pare
     beam step may permute and branch rows in place.  block_tables [R, MB], context_lens [R] and
     page_refs [NB] (holders per page, 0 = free) are int32 and updated in place.  Returns int32 [N]:
     the page each begun page was copied to, -1 none needed, -2 no page free, -3 refused."""
-    _state(block_tables, context_lens, page_refs)
-    dev = block_tables.device
-    return _native().fork_sequences(_pages(k_cache), _pages(v_cache), block_tables, context_lens, page_refs,
-                                    parents.to(dev, torch.int32).contiguous(), rows.to(dev, torch.int32).contiguous())
+    return _native().fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows)
 
 
 def free_sequences(block_tables, context_lens, page_refs, rows, block_size):
     """Rows of the block tables let go of their pages and end empty, in place (pa_free_sequences)."""
-    _state(block_tables, context_lens, page_refs)
-    _native().free_sequences(block_tables, context_lens, page_refs,
-                             rows.to(block_tables.device, torch.int32).contiguous(), int(block_size))
+    _native().free_sequences(block_tables, context_lens, page_refs, rows, block_size)
 
 
 def compact_pages(k_cache, v_cache, block_tables, page_refs, *, tables_out=None, refs_out=None):
@@ -450,10 +452,9 @@ def compact_pages(k_cache, v_cache, block_tables, page_refs, *, tables_out=None,
     as a dense cache allows, and brings block_tables and page_refs in line: in place, or into
     tables_out / refs_out (pa_compact_pages).  Returns (page_map [NB]: each page's place now, -1 for
     a free one; num_live [1]), int32 on the GPU."""
-    tables_out = block_tables if tables_out is None else tables_out
-    refs_out = page_refs if refs_out is None else refs_out
-    _state(block_tables, page_refs, tables_out, refs_out)
-    return _native().compact_pages(_pages(k_cache), _pages(v_cache), block_tables, page_refs, tables_out, refs_out)
+    return _native().compact_pages(k_cache, v_cache, block_tables, page_refs,
+                                   block_tables if tables_out is None else tables_out,
+                                   page_refs if refs_out is None else refs_out)
 
 
 _ops = None

@@ -326,3 +326,47 @@ def test_captured(pa, dev):
         torch.cuda.synchronize()
         for x, y in zip(got, want):
             assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+def test_python_paths_agree(pa, dev, monkeypatch, tmp_path):
+    """Without the operator library: the same state, results and refusals."""
+    import sys
+    ops = sys.modules[pa.paged_attention.__module__]
+
+    def calls():
+        bt, ctx, refs = state(9, 6, 64, 4, [21, 10, 7], np.random.default_rng(8))
+        data = pool(2, 64, 4, 1, 32, "bf16", dev)
+        st = [torch.from_numpy(x).to(dev) for x in (bt, ctx, refs)]
+        new = pa.fork_sequences(data[:, 0], data[:, 1], *st, torch.tensor([0, 1, 2, 0]), torch.tensor([3, 4, 5, 6]))
+        pa.free_sequences(*st, torch.tensor([1, 4], device=dev), 4)
+        where, n = pa.compact_pages(data[:, 0], data[:, 1], st[0], st[2])
+        pa.copy_pages(data[:, 0], data[:, 1], torch.tensor([0, 1]), torch.tensor([60, 61]))
+        pa.copy_pages(data[1, 0], None, torch.tensor([2]), torch.tensor([62]))
+        return [new, where, n, *st, data.view(torch.int16)]
+
+    def refusals():
+        data = pool(1, 8, 4, 2, 32, "f16", dev)
+        st = [torch.zeros(s, dtype=torch.int32, device=dev) for s in ((2, 2), (2,), (8,))]
+        one = torch.tensor([0], device=dev)
+        with pytest.raises(RuntimeError, match="must be int32 on CUDA"):
+            pa.fork_sequences(data[:, 0], data[:, 1], st[0].long(), *st[1:], one, one)
+        with pytest.raises(RuntimeError, match="must be int32 on CUDA"):
+            pa.compact_pages(data[:, 0], data[:, 1], st[0], st[2].cpu())
+        with pytest.raises(RuntimeError, match="contiguous token rows"):
+            pa.copy_pages(data[0, 0].transpose(1, 2), None, one, one)
+        with pytest.raises(RuntimeError, match=r"\[NB, BS, HKV, D\]"):
+            pa.copy_pages(data, None, one, one)
+        with pytest.raises(RuntimeError, match="on CUDA"):
+            pa.copy_pages(data[:, 0].cpu(), None, one, one)
+        with pytest.raises(RuntimeError, match="parents must have 1 entries"):
+            pa.fork_sequences(data[:, 0], data[:, 1], *st, one.repeat(2), one)
+
+    print("python paths", flush=True)
+    want = calls()
+    refusals()
+    monkeypatch.setattr(ops, "_ops", None)
+    monkeypatch.setattr(ops, "_torch_path", lambda: tmp_path / "none.so")
+    assert ops._native() is ops._CAbi
+    for x, y in zip(calls(), want):
+        assert torch.equal(x, y)
+    refusals()

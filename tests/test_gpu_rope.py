@@ -201,3 +201,42 @@ def test_captured_and_on_a_stream(pa, dev):
         want = call()
         torch.cuda.synchronize()
         assert torch.equal(got[0], want) and torch.equal(got[1], kc)
+
+
+def test_python_paths_agree(pa, dev, monkeypatch, tmp_path):
+    """Without the operator library, on copies and views: the same results and refusals."""
+    import sys
+    ops = sys.modules[pa.paged_attention.__module__]
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn((9, n, 64), generator=g).bfloat16().to(dev) for n in (4, 2, 2))
+    w = torch.randn(64, generator=g).to(dev)
+    cs = table(32, 32, torch.float32).to(dev)
+    pos, slots = torch.arange(9), torch.arange(9, dtype=torch.int16) * 3
+
+    def calls():
+        kc, vc = (torch.zeros((3, 16, 2, 64), dtype=torch.float8_e4m3fn, device=dev) for _ in range(2))
+        odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=dev)[1:].view(q.shape).copy_(q)  # not 16-byte aligned
+        wide = k.repeat_interleave(2, 2)[..., ::2]                                              # last dim strided
+        a = pa.qk_norm_rope_write_kv(odd, wide, v, kc, vc, slots, cs, pos, q_weight=w, k_weight=w, k_scale=0.5)
+        b = pa.qk_norm_rope_write_kv(q, k, v, kc, vc, slots.to(dev) + 1, cs, pos.to(dev), out_dtype=torch.float32)
+        return [a, b, kc.view(torch.uint8), vc.view(torch.uint8)]
+
+    def refusals():
+        kc = torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16, device=dev)
+        with pytest.raises(RuntimeError, match="key must be on CUDA"):
+            pa.qk_norm_rope_write_kv(q, k.cpu(), v, kc, kc.clone(), slots, cs, pos)
+        with pytest.raises(RuntimeError, match=r"q must be \[T, H, D\]"):
+            pa.qk_norm_rope_write_kv(q[0], k, v, kc, kc.clone(), slots, cs, pos)
+        with pytest.raises(RuntimeError, match="16-byte aligned"):
+            pa.qk_norm_rope_write_kv(q, k, v, kc.transpose(2, 3), kc.clone(), slots, cs, pos)
+        with pytest.raises(RuntimeError, match="positions must have 9 entries"):
+            pa.qk_norm_rope_write_kv(q, k, v, kc, kc.clone(), slots, cs, pos[:8])
+
+    print("python paths", flush=True)
+    want = calls()
+    refusals()
+    monkeypatch.setattr(ops, "_ops", None)
+    monkeypatch.setattr(ops, "_torch_path", lambda: tmp_path / "none.so")
+    for x, y in zip(calls(), want):
+        assert x.dtype == y.dtype and torch.equal(x, y)
+    refusals()
