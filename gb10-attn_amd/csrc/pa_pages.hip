@@ -8,7 +8,9 @@
 //
 //  * The data moves as bytes, 16 a load: HBM-bound, each page read and written
 //    once.  A work item is kPiece pieces of one page on one plane (a layer's K
-//    or V); a thread has kDepth pieces in flight.
+//    or V); a thread has kDepth pieces in flight.  256 pages of 12 layers (201 MB)
+//    move in 39.6 us, a compaction's 245 pages (289 MB) in 59.5: 5.1 and 4.9 TB/s
+//    read + write, where a copy of 1 GB runs at 5.1.
 //  * The bookkeeping is exact and independent of the order in which work-groups
 //    run: counts change by integer atomics whose sum is all that matters, and
 //    whatever is handed out goes by index (the lowest free page to the first
@@ -89,11 +91,11 @@ hipError_t launch_copy_pages(const CopyParams& p, hipStream_t stream) {
 
 // ------------------------------------------------------------------- fork --
 
-// Whether entry i is the first that names its row.
+// Whether entry i is the first that names its row (a wave's lanes search together).
 __device__ inline bool first_of_row(const int32_t* rows, int i, int32_t row) {
-  int again = 0;
-  for (int j = threadIdx.x; j < i; j += kPgThreads) again |= rows[j] == row;
-  return !__syncthreads_or(again);
+  bool again = false;
+  for (int j = threadIdx.x & 63; j < i; j += 64) again |= rows[j] == row;
+  return __builtin_amdgcn_ballot_w64(again) == 0;
 }
 
 // Pages a row holds: those of its context, or none where it exceeds the table.
@@ -101,16 +103,15 @@ __device__ inline int pages_of(const ForkParams& p, int32_t len) {
   return len > 0 && (int64_t)len <= (int64_t)p.MB * p.BS ? (int)fastdiv((uint32_t)(len - 1), p.bs_div) + 1 : 0;
 }
 
-// One work-group per entry: the row's old pages are let go, the parent's whole
-// pages are counted once more and its pages kept aside, since another entry may
-// replace the parent's own row.  No table changes yet.
-__global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams p) {
-  const int i = blockIdx.x;
+// One wave's entry: the row's old pages are let go, the parent's whole pages are
+// counted once more and its pages kept aside, since another entry may replace the
+// parent's own row.  No table changes yet.
+__device__ inline void share_entry(const ForkParams& p, int i) {
+  const int lane = threadIdx.x & 63;
   const int32_t row = p.rows[i];
   const int64_t NB = p.pool.num_blocks;
-  const bool inside = row >= 0 && row < p.R;
-  if (!first_of_row(p.rows, i, row) || !inside) {  // (every thread takes the test's barrier)
-    if (threadIdx.x == 0) {
+  if (row < 0 || row >= p.R || !first_of_row(p.rows, i, row)) {
+    if (lane == 0) {
       p.ws_len[i] = -1;
       p.ws_last[i] = -1;
       p.result[i] = kForkInvalid;
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams
   }
   const int32_t* old = p.tables + row * p.tb_stride;
   const int held = pages_of(p, p.lens[row]);
-  for (int j = threadIdx.x; j < held; j += kPgThreads) {
+  for (int j = lane; j < held; j += 64) {
     const int32_t pg = old[j];
     if (pg >= 0 && pg < NB) atomicAdd(p.refs + pg, -1);
   }
@@ -131,26 +132,30 @@ __global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams
     len = max(p.lens[par], 0);
     const int n = pages_of(p, len);
     const int32_t* src = p.tables + par * p.tb_stride;
-    int bad = len > 0 && n == 0;
-    for (int j = threadIdx.x; j < n; j += kPgThreads) bad |= src[j] < 0 || src[j] >= NB;
-    bad = __syncthreads_or(bad);
-    if (bad) {
+    bool bad = len > 0 && n == 0;
+    for (int j = lane; j < n; j += 64) bad |= src[j] < 0 || src[j] >= NB;
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
       len = 0;
       res = kForkInvalid;
     } else {
       const int whole = (int)fastdiv((uint32_t)len, p.bs_div);
-      for (int j = threadIdx.x; j < n; j += kPgThreads) {
+      for (int j = lane; j < n; j += 64) {
         p.ws_pages[(int64_t)i * p.MB + j] = src[j];
         if (j < whole) atomicAdd(p.refs + src[j], 1);
       }
       if (whole < n) last = src[whole];
     }
   }
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     p.ws_len[i] = len;
     p.ws_last[i] = last;
     p.result[i] = res;
   }
+}
+
+__global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams p) {
+  const int i = blockIdx.x * (kPgThreads / 64) + (threadIdx.x >> 6);
+  if (i < p.N) share_entry(p, i);
 }
 
 // Exclusive prefix sum over the work-group's kScan threads, and the total.
@@ -176,14 +181,20 @@ __device__ inline int scan_block(int v, int& total, int* s_part) {
   return before + x - v;
 }
 
-// One work-group.  A begun page that nobody holds any more goes to the lowest
+// One work-group (kShare: with share_entry() of every entry first, which saves a launch
+// where there are few table entries to walk).  A begun page that nobody holds any more goes to the lowest
 // entry forked from it; every other entry with a begun page gets a copy, in the
 // lowest free page, in the order of the entries.  Free pages are found in one
 // pass over the counts that ends when there are enough.
+template <bool kShare>
 __global__ __launch_bounds__(kScan) void fork_alloc_kernel(const ForkParams p) {
   __shared__ int s_part[kScan / 64];
   const int tid = threadIdx.x;
   const int64_t NB = p.pool.num_blocks;
+  if constexpr (kShare) {
+    for (int i = tid >> 6; i < p.N; i += kScan / 64) share_entry(p, i);
+    __syncthreads();
+  }
   for (int i = tid; i < p.N; i += kScan) {
     const int32_t last = p.ws_last[i];
     if (last >= 0) atomicExch(p.ws_owner + last, INT32_MAX);
@@ -284,33 +295,42 @@ __global__ __launch_bounds__(kPgThreads) void fork_write_kernel(const ForkParams
 
 // Rows emptied without a cache or workspace: one launch.
 __global__ __launch_bounds__(kPgThreads) void free_kernel(const ForkParams p) {
-  const int i = blockIdx.x;
+  const int i = blockIdx.x * (kPgThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= p.N) return;
   const int32_t row = p.rows[i];
-  if (!first_of_row(p.rows, i, row) || row < 0 || row >= p.R) return;
+  if (row < 0 || row >= p.R || !first_of_row(p.rows, i, row)) return;
   int32_t* t = p.tables + row * p.tb_stride;
   const int held = pages_of(p, p.lens[row]);
-  __syncthreads();  // every thread has the length
-  for (int j = threadIdx.x; j < p.MB; j += kPgThreads) {
+  for (int j = lane; j < p.MB; j += 64) {
     const int32_t pg = t[j];
     if (j < held && pg >= 0 && pg < p.pool.num_blocks) atomicAdd(p.refs + pg, -1);
     t[j] = -1;
   }
-  if (threadIdx.x == 0) p.lens[row] = 0;
+  if (lane == 0) p.lens[row] = 0;
 }
 
 hipError_t launch_free(const ForkParams& p, hipStream_t stream) {
   note_launch("pa::free_kernel");
-  hipLaunchKernelGGL(free_kernel, dim3(p.N), dim3(kPgThreads), 0, stream, p);
+  hipLaunchKernelGGL(free_kernel, dim3((unsigned)((p.N + 3) / 4)), dim3(kPgThreads), 0, stream, p);
   return hipGetLastError();
 }
 
+// Most table entries that one work-group walks for a fork: 8 entries of tables of 16
+// pages 13.1 us in three launches, 11.0 in two; 64 of 128 22.8, and 37.8 in two.
+constexpr int64_t kForkFused = 1024;
+
 hipError_t launch_fork(const ForkParams& p, hipStream_t stream) {
-  note_launch("pa::fork_share_kernel");
-  hipLaunchKernelGGL(fork_share_kernel, dim3(p.N), dim3(kPgThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  note_launch("pa::fork_alloc_kernel");
-  hipLaunchKernelGGL(fork_alloc_kernel, dim3(1), dim3(kScan), 0, stream, p);
+  hipError_t e;
+  if ((int64_t)p.N * p.MB <= kForkFused) {
+    note_launch("pa::fork_alloc_kernel<true>");
+    hipLaunchKernelGGL(fork_alloc_kernel<true>, dim3(1), dim3(kScan), 0, stream, p);
+  } else {
+    note_launch("pa::fork_share_kernel");
+    hipLaunchKernelGGL(fork_share_kernel, dim3((unsigned)((p.N + 3) / 4)), dim3(kPgThreads), 0, stream, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    note_launch("pa::fork_alloc_kernel<false>");
+    hipLaunchKernelGGL(fork_alloc_kernel<false>, dim3(1), dim3(kScan), 0, stream, p);
+  }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int64_t copies = std::min<int64_t>((int64_t)p.N * p.pool.planes * page_items(p.pool), kMaxGrid);
   note_launch("pa::fork_write_kernel");
@@ -333,6 +353,22 @@ __device__ inline int block_sum(int v, int* s_part) {
   if (lane == 0) s_part[threadIdx.x >> 6] = v;
   __syncthreads();
   return s_part[0] + s_part[1] + s_part[2] + s_part[3];
+}
+
+// Page `pg` of count r: `all` pages live in all, `below` of them before page `all`,
+// `before` before this one (moved on).  A moved page's map entry holds its number in
+// the order of the moves, as -2 - number, until the move writes where it goes.
+__device__ inline void place_page(const CompactParams& p, int pg, int32_t r, int all, int below, int& before) {
+  const bool live = r > 0;
+  if (pg < all) {
+    if (!live) p.ws_to[pg - before] = pg;
+    p.page_map[pg] = live ? pg : -1;
+  } else {
+    if (live) p.ws_from[before - below] = pg;
+    p.page_map[pg] = live ? -2 - (before - below) : -1;
+  }
+  p.refs_out[pg] = r;
+  before += live;
 }
 
 __global__ __launch_bounds__(kPgThreads) void compact_count_kernel(const CompactParams p) {
@@ -393,21 +429,51 @@ __global__ __launch_bounds__(kPgThreads) void compact_map_kernel(const CompactPa
   for (int k = 0; k < kCompactPer; ++k) {
     const int64_t pg = first + k;
     if (pg >= NB) break;
-    const bool live = r[k] > 0;
-    if (pg < all) {
-      if (!live) p.ws_to[pg - before] = (int32_t)pg;
-      p.page_map[pg] = live ? (int32_t)pg : -1;
-      p.refs_out[pg] = r[k];
-    } else {
-      // A moved page's entry holds its number in the order of the moves, as -2 -
-      // number, until the move writes where it goes.
-      if (live) p.ws_from[before - below] = (int32_t)pg;
-      p.page_map[pg] = live ? -2 - (before - below) : -1;
-      p.refs_out[pg] = r[k];
-    }
-    before += live;
+    place_page(p, (int)pg, r[k], all, below, before);
   }
   if (blockIdx.x == 0 && tid == 0) {
+    p.ws_moves[0] = all - below;
+    p.num_live[0] = all;
+  }
+}
+
+// The same for few pages, in one launch of one work-group: kPlanPer consecutive
+// pages of a thread (128 pages 12.9 -> 9.8 us a call).
+constexpr int kPlanPer = 8;
+constexpr int kPlanPages = kScan * kPlanPer;
+
+__global__ __launch_bounds__(kScan) void compact_plan_kernel(const CompactParams p) {
+  __shared__ int s_part[kScan / 64];
+  __shared__ int s_below;
+  const int NB = (int)p.pool.num_blocks, first = threadIdx.x * kPlanPer;
+  int32_t r[kPlanPer];
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    r[k] = first + k < NB ? p.refs[first + k] : 0;
+    n += r[k] > 0;
+  }
+  int all;
+  const int start = scan_block(n, all, s_part);
+  // Live pages before page `all`.
+  if (threadIdx.x == 0) s_below = all;  // (none after it, unless a thread finds it)
+  __syncthreads();
+  if (all >= first && all < first + kPlanPer) {
+    int below = start;
+#pragma unroll
+    for (int k = 0; k < kPlanPer; ++k) below += first + k < all && r[k] > 0;
+    s_below = below;
+  }
+  __syncthreads();
+  const int below = s_below;
+  int before = start;
+#pragma unroll
+  for (int k = 0; k < kPlanPer; ++k) {
+    const int pg = first + k;
+    if (pg >= NB) break;
+    place_page(p, pg, r[k], all, below, before);
+  }
+  if (threadIdx.x == 0) {
     p.ws_moves[0] = all - below;
     p.num_live[0] = all;
   }
@@ -446,12 +512,17 @@ __global__ __launch_bounds__(kPgThreads) void compact_move_kernel(const CompactP
 }
 
 hipError_t launch_compact(const CompactParams& p, hipStream_t stream) {
-  note_launch("pa::compact_count_kernel");
-  hipLaunchKernelGGL(compact_count_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  note_launch("pa::compact_map_kernel");
-  hipLaunchKernelGGL(compact_map_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
+  hipError_t e;
+  if (p.pool.num_blocks <= kPlanPages) {
+    note_launch("pa::compact_plan_kernel");
+    hipLaunchKernelGGL(compact_plan_kernel, dim3(1), dim3(kScan), 0, stream, p);
+  } else {
+    note_launch("pa::compact_count_kernel");
+    hipLaunchKernelGGL(compact_count_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    note_launch("pa::compact_map_kernel");
+    hipLaunchKernelGGL(compact_map_kernel, dim3(p.blocks), dim3(kPgThreads), 0, stream, p);
+  }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   // At most half of the pages move.
   const int64_t work = std::max<int64_t>((p.pool.num_blocks / 2 + 1) * p.pool.planes * page_items(p.pool),

@@ -203,7 +203,8 @@ def test_free(pa, dev):
 
 
 @pytest.mark.parametrize("NB,live", [(1, 1.0), (3, 0.0), (64, 0.4), (64, 1.0), (2047, 0.5), (2048, 0.9), (2049, 0.05),
-                                     (9000, 0.3), (4096, 0.5)])
+                                     (8192, 0.4), (8193, 0.6), (9000, 0.3), (20000, 0.5), (4096, 0.5), (8192, 1.0),
+                                     (8192, 0.0), (10240, 1.0)])
 def test_compact(pa, dev, NB, live):
     rng = np.random.default_rng(NB)
     L, BS, HKV, D = 2, 4, 1, 32
