@@ -1343,6 +1343,13 @@ extern "C" int pa_qk_norm_rope_write_kv(pa_tensor_t* q_out, pa_tensor_t* k_cache
       (rc = check_rows(value, "value", 2)) || (rc = check_rows(k_cache, "k_cache", 3)) ||
       (rc = check_rows(v_cache, "v_cache", 3)) || (rot > 0 && (rc = check_rows(cos_sin, "cos_sin", 1))))
     return rc;
+  for (int i = 0; i < 2; ++i)
+    if (q_out->shape[i] > 1 && q_out->stride[i] == 0)
+      return fail(PA_ERR_INVALID_ARGUMENT, "q_out's rows must not overlap");
+  for (const pa_tensor_t* t : {k_cache, v_cache})
+    for (int i = 0; i < 3; ++i)
+      if (t->shape[i] > 1 && t->stride[i] == 0)
+        return fail(PA_ERR_INVALID_ARGUMENT, "k_cache/v_cache rows must not overlap");
   if (T == 0 || H + HKV == 0) return PA_OK;
   RopeParams p;
   memset(&p, 0, sizeof(p));
@@ -1468,7 +1475,8 @@ extern "C" int pa_copy_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const p
   if ((rc = check_pool(k_cache, v_cache, &p.pool)) || (rc = check_index(src, "src", -1, false)) ||
       (rc = check_index(dst, "dst", src->shape[0], false)))
     return rc;
-  if (src->shape[0] >= (1LL << 24)) return fail(PA_ERR_UNSUPPORTED, "too many pages for one call");
+  // (A work-group looks through the later pairs for its destination.)
+  if (src->shape[0] > kForkMax) return fail(PA_ERR_UNSUPPORTED, "at most %lld pages per call", (long long)kForkMax);
   p.src = static_cast<const int32_t*>(src->data);
   p.dst = static_cast<const int32_t*>(dst->data);
   p.N = (int32_t)src->shape[0];
@@ -1590,6 +1598,9 @@ extern "C" int pa_compact_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, cons
 static int plan_shared(SharedParams* p) {
   if (p->B > kSharedMaxSeqs || p->NG > kSharedMaxGroups)
     return fail(PA_ERR_UNSUPPORTED, "at most %d sequences and %d groups", kSharedMaxSeqs, kSharedMaxGroups);
+  // (A unit's last tile may end past its keys.)
+  if ((int64_t)p->MB * p->BS >= (1LL << 31) - 1024)
+    return fail(PA_ERR_UNSUPPORTED, "block tables too long for 32-bit token indices");
   int cus = 0, rc;
   if ((rc = device_cu_count(&cus))) return rc;
   const int64_t sg = (int64_t)p->S * p->G, rows = p->B * sg;

@@ -255,7 +255,7 @@ struct PagePool {
 };
 
 constexpr int64_t kMaxPiece = 1024;  // 16-byte pieces of a page that a work-group moves at a time
-constexpr int64_t kForkMax = 65536;  // most rows of a fork or a release
+constexpr int64_t kForkMax = 65536;  // most rows of a fork or a release, and pairs of a copy
 
 struct CopyParams {
   PagePool pool;

@@ -298,9 +298,10 @@ std::optional<at::Tensor> rows_of(const std::optional<at::Tensor>& t) {
 }
 
 // Integer vectors as the entry points take them: int32 or int64 (int32 alone with
-// `narrow`), contiguous, on the device.
+// `narrow`: what does not fit stays out of range), contiguous, on the device.
 at::Tensor index_of(const at::Tensor& t, const at::Device& dev, bool narrow) {
   const at::ScalarType ty = t.scalar_type();
+  if (narrow && ty == at::kLong) return t.to(dev).clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
   const at::ScalarType want = narrow ? at::kInt : ty == at::kInt || ty == at::kLong ? ty : at::kLong;
   return t.to(dev, want).contiguous();
 }
@@ -341,9 +342,8 @@ void op_shared_prefix_out(const at::Tensor& q, const at::Tensor& k, const at::Te
                           double scale, double k_scale, double v_scale, const at::Tensor& out) {
   Args a = q.dim() == 3 ? prep(q, k, v, bt, ctx, 3, "[B, H, D]") : prep(q, k, v, bt, ctx, 4, "[B, S, H, D]");
   if (reinterpret_cast<uintptr_t>(a.q.data_ptr()) % 16) a.q = a.q.clone();
-  at::Tensor gs = group_starts.to(a.q.device(), at::kInt).contiguous();
-  at::Tensor pl = prefix_lens.to(a.q.device(), at::kInt).contiguous();
   c10::DeviceGuard guard(a.q.device());
+  const at::Tensor gs = index_of(group_starts, a.q.device(), true), pl = index_of(prefix_lens, a.q.device(), true);
   pa_tensor_t o = view(out), qq = view(a.q), kk = view(a.k), vv = view(a.v), bb = view(a.bt), cc = view(a.ctx),
               gg = view(gs), pp = view(pl);
   Scratch s = scratch_of(a.q, paged_attention_shared_prefix_workspace_size(&qq, &kk, &bb, &gg));

@@ -140,6 +140,7 @@ class _CAbi:
         o = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device) if out is None else out
         q, key, value, cos_sin = (_rows(t) for t in (q, key, value, cos_sin))
         q_weight, k_weight = (t if t is None else _rows(t) for t in (q_weight, k_weight))
+        _one_device(q, key, value, k_cache, v_cache, cos_sin, o, q_weight, k_weight)
         slot_mapping, positions = (_index(t, q.device) for t in (slot_mapping, positions))
         with torch.cuda.device(q.device):
             check(lib().pa_qk_norm_rope_write_kv(*_refs(o, k_cache, v_cache, q, key, value, slot_mapping, cos_sin,
@@ -153,7 +154,7 @@ class _CAbi:
         args = _prep(q, k_cache, v_cache, block_tables, context_lens, *((3, "[B, H, D]") if q.dim() == 3
                                                                         else (4, "[B, S, H, D]")))
         q = args[0] if args[0].data_ptr() % 16 == 0 else args[0].clone()
-        starts, lens = (t.to(q.device, torch.int32).contiguous() for t in (group_starts, prefix_lens))
+        starts, lens = (_index(t, q.device, True) for t in (group_starts, prefix_lens))
         with torch.cuda.device(q.device):
             need = lib().paged_attention_shared_prefix_workspace_size(*_refs(q, args[1], args[3], starts))
             ws = _scratch(need, q.device)
@@ -163,15 +164,16 @@ class _CAbi:
     @staticmethod
     def copy_pages(k_cache, v_cache, src, dst):
         k = _pages(k_cache)
-        src, dst = (t.to(k.device, torch.int32).contiguous() for t in (src, dst))
+        _one_device(k_cache, v_cache)
+        src, dst = (_index(t, k.device, True) for t in (src, dst))
         with torch.cuda.device(k.device):
             check(lib().pa_copy_pages(*_refs(k, _pages(v_cache), src, dst), _stream(k.device)))
 
     @staticmethod
     def fork_sequences(k_cache, v_cache, block_tables, context_lens, page_refs, parents, rows):
         _state(block_tables, context_lens, page_refs)
-        dev = block_tables.device
-        parents, rows = (t.to(dev, torch.int32).contiguous() for t in (parents, rows))
+        dev = _one_device(k_cache, v_cache, block_tables, context_lens, page_refs)
+        parents, rows = (_index(t, dev, True) for t in (parents, rows))
         copied = torch.empty(rows.shape, dtype=torch.int32, device=dev)
         with torch.cuda.device(dev):
             ws = _scratch(lib().pa_fork_workspace_size(*_refs(block_tables, page_refs, rows)), dev)
@@ -182,15 +184,15 @@ class _CAbi:
     @staticmethod
     def free_sequences(block_tables, context_lens, page_refs, rows, block_size):
         _state(block_tables, context_lens, page_refs)
-        dev = block_tables.device
-        rows = rows.to(dev, torch.int32).contiguous()
+        dev = _one_device(block_tables, context_lens, page_refs)
+        rows = _index(rows, dev, True)
         with torch.cuda.device(dev):
             check(lib().pa_free_sequences(*_refs(block_tables, context_lens, page_refs, rows), block_size, _stream(dev)))
 
     @staticmethod
     def compact_pages(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out):
         _state(block_tables, page_refs, tables_out, refs_out)
-        dev = page_refs.device
+        dev = _one_device(k_cache, v_cache, block_tables, page_refs, tables_out, refs_out)
         page_map, n = torch.empty_like(page_refs), torch.empty(1, dtype=torch.int32, device=dev)
         with torch.cuda.device(dev):
             ws = _scratch(lib().pa_compact_workspace_size(*_refs(page_refs)), dev)
@@ -395,10 +397,19 @@ def _rows(t):
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
-def _index(t, dev):
-    if t.dtype not in (torch.int32, torch.int64):
-        t = t.to(torch.int64)
+def _index(t, dev, narrow=False):
+    """An integer vector on the device: int32 or int64, or int32 alone (what does not fit stays out of range)."""
+    if narrow and t.dtype == torch.int64:
+        t = t.to(dev).clamp(-2**31, 2**31 - 1)
+    if narrow or t.dtype not in (torch.int32, torch.int64):
+        t = t.to(torch.int32 if narrow else torch.int64)
     return t.to(dev).contiguous()
+
+
+def _one_device(first, *others):
+    if any(t is not None and t.device != first.device for t in others):
+        raise RuntimeError("all tensors must be on one device")
+    return first.device
 
 
 def _pages(t):

@@ -348,7 +348,8 @@ int pa_write_kv_scaled(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tens
  * rows; a row that attends an unreadable page, whose context or prefix exceeds MB *
  * BS tokens, and every row where group_starts decreases or leaves [0, B], is NaN.
  * fp16, bf16 or FP8 E4M3 caches (k_scale, v_scale as the scaled entry points), q and
- * out fp32, fp16 or bf16, q 16-byte aligned, B <= 1024, NG <= 512, D in {32, 64, 128, 256}.
+ * out fp32, fp16 or bf16, q 16-byte aligned, B <= 1024, NG <= 512, MB * BS < 2^31 - 1024,
+ * D in {32, 64, 128, 256}.
  * Probabilities are carried in 16 bits where out is a 16-bit type, as 16-bit hi + lo
  * pairs where it is fp32 (an infinite V element may then give NaN in its place).
  * workspace: device memory of paged_attention_shared_prefix_workspace_size(...)
@@ -400,7 +401,7 @@ int pa_qk_norm_rope_write_kv(pa_tensor_t* q_out, pa_tensor_t* k_cache, pa_tensor
 /* Pages src[i] -> dst[i] (int32 [N]) of every layer.  Pairs with a page outside the
  * pool are skipped; a destination named twice takes the last pair that names it.
  * A page that is both a source and a destination has unspecified contents in the
- * pages copied from it. */
+ * pages copied from it.  At most 65536 pairs. */
 int pa_copy_pages(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tensor_t* src, const pa_tensor_t* dst,
                   void* stream);
 

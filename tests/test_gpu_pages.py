@@ -371,3 +371,26 @@ def test_python_paths_agree(pa, dev, monkeypatch, tmp_path):
     for x, y in zip(calls(), want):
         assert torch.equal(x, y)
     refusals()
+
+
+def test_numbers_past_32_bits(pa, dev, monkeypatch, tmp_path):
+    """int64 pages and rows that do not fit are outside, not what is left of them in 32 bits."""
+    import sys
+    ops = sys.modules[pa.paged_attention.__module__]
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(ops, "_ops", None)
+            monkeypatch.setattr(ops, "_torch_path", lambda: tmp_path / "none.so")
+        data = pool(1, 8, 4, 1, 32, "bf16", dev)
+        first = data.clone()
+        print("wide indices", native, flush=True)
+        pa.copy_pages(data[0, 0], data[0, 1], torch.tensor([2**32, 1, 3, -2**32 + 4]), torch.tensor([5, 2**32 + 6, 7, 2]))
+        first[:, :, 7] = first[:, :, 3]
+        assert torch.equal(data.view(torch.uint8), first.view(torch.uint8))
+        bt, ctx, refs = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([[0, 1], [-1, -1], [-1, -1]], [8, 0, 0],
+                                                                                  [1, 1, 0, 0, 0, 0, 0, 0]))
+        got = pa.fork_sequences(data[:, 0], data[:, 1], bt, ctx, refs, torch.tensor([2**32, 0, -2**32]),
+                                torch.tensor([1, 2**32 + 2, 2]))
+        assert got.tolist() == [-3, -3, -1] and ctx.tolist() == [8, 0, 0] and refs.tolist() == [1, 1] + [0] * 6
+        pa.free_sequences(bt, ctx, refs, torch.tensor([2**32, -2**33]), 4)
+        assert ctx.tolist() == [8, 0, 0] and refs.tolist() == [1, 1] + [0] * 6

@@ -335,3 +335,41 @@ def test_python_paths_agree(pa, dev, monkeypatch, tmp_path):
     monkeypatch.setattr(ops, "_torch_path", lambda: tmp_path / "none.so")
     assert torch.equal(pa.paged_attention_shared_prefix(*wide, 0.125), want)
     assert torch.equal(pa.paged_attention_shared_prefix(off, *t[1:], 0.125), want)
+
+
+def test_numbers_past_32_bits(pa, dev, monkeypatch, tmp_path):
+    """int64 group starts and prefixes that do not fit are out of range."""
+    import sys
+    ops = sys.modules[pa.paged_attention.__module__]
+    c = case(4, 8, 2, 64, 16, [0, 4], [32], [40, 41, 50, 33], kv="bf16", q="bf16")
+    t = [c[n].to(dev) for n in ("q", "k", "v", "bt", "ctx")]
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(ops, "_ops", None)
+            monkeypatch.setattr(ops, "_torch_path", lambda: tmp_path / "none.so")
+        print("wide numbers", native, flush=True)
+        for starts, prefix in (([2**32, 4], [32]), ([0, 2**32 + 4], [32]), ([0, 4], [2**32 + 32])):
+            got = pa.paged_attention_shared_prefix(*t, torch.tensor(starts), torch.tensor(prefix), 0.125)
+            assert got.isnan().all()
+
+
+def test_long_table(pa, dev):
+    """A table near the longest that a call takes, on few pages."""
+    MB = (1 << 27) - 128
+    k, v = (torch.randn((3, 16, 1, 32), device=dev).half() for _ in range(2))
+    q = torch.randn((1, 1, 32), device=dev).half()
+    bt = torch.ones((1, MB), dtype=torch.int32, device=dev)
+    print("long table", flush=True)
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    short = pa.paged_attention_shared_prefix(q, k, v, bt[:, :1].clone(), i([16]), i([0, 1]), i([0]), 0.1)
+    for n, P in ((16, 0), (MB * 16 + 1, 0)):
+        got = pa.paged_attention_shared_prefix(q, k, v, bt, i([n]), i([0, 1]), i([P]), 0.1)
+        assert got.isnan().all() if n > MB * 16 else torch.equal(got, short)
+    # Every page alike: the mean over a page's keys stays.  The first half goes to wide work-groups, the second
+    # to thin ones, an equal cost each: a row's state sums at most 61 k keys of 2^25 (946 tiles of 64), one
+    # rounding of 2^-24 a key in the products and half as many in the weights' sum, and the merge adds 2600
+    # states.  Together below 2^-7.  64 times as many keys: below 1/2.
+    for n, tol in ((1 << 25, 2.0**-7), (MB * 16, 0.5)):
+        print("tokens", n, flush=True)
+        got = pa.paged_attention_shared_prefix(q, k, v, bt[:, :n // 16].clone(), i([n]), i([0, 1]), i([n // 2]), 0.1)
+        assert (got - short).abs().max() <= tol * v.float().abs().max()

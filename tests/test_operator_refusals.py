@@ -248,3 +248,29 @@ def test_shared_prefix_scalars_and_null(pa):
     for sizes in (dict(B=1025), dict(NG=513), dict(H=9), dict(D=512)):
         b = shared_args(pa, **sizes)
         assert size(*refs(b[n] for n in ("q", "k", "bt", "starts"))) == C.c_size_t(-1).value
+
+
+# ------------------------------------------------------------ limits and overlaps --
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(q_out=([5, 4, 64], BF16, [0, 64, 1])), "q_out's rows must not overlap"),
+    (dict(q_out=([5, 4, 64], BF16, [256, 0, 1])), "q_out's rows must not overlap"),
+    (dict(k_cache=([10, 16, 2, 64], F16, [0, 128, 64, 1])), "k_cache/v_cache rows must not overlap"),
+    (dict(v_cache=([10, 16, 2, 64], F16, [2048, 128, 0, 1])), "k_cache/v_cache rows must not overlap"),
+])
+def test_rope_outputs_that_overlap(pa, change, msg):
+    a = rope_args(pa)
+    for n, s in change.items():
+        a[n] = T(pa, *s)
+    expect(pa, rope_call(pa, a), 1, msg)
+
+
+def test_limits_of_one_call(pa):
+    a = page_args(pa, N=65537)
+    expect(pa, copy_call(pa, a), 2, "at most 65536 pages")
+    # A table that reaches the last 32-bit token: a unit's last tile would pass it.
+    for MB in ((1 << 27) - 1, (1 << 27) - 64):
+        b = shared_args(pa, B=1, H=1, HKV=1, NG=1, MB=MB)
+        expect(pa, shared_call(pa, b), 2, "block tables too long for 32-bit token indices")
+        size = pa.lib().paged_attention_shared_prefix_workspace_size(*refs(b[n] for n in ("q", "k", "bt", "starts")))
+        assert size == C.c_size_t(-1).value
