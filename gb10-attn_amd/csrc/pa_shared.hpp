@@ -29,9 +29,10 @@
 // O^T += V^T P^T: the probabilities stay in registers.
 //
 // Types.  FP8 codes widen exactly to the 16-bit type of q.  q of another type than
-// the tiles' is carried as hi + lo; the probabilities as hi + lo where the output is
-// fp32 (2^-17 of bf16 pieces, 2^-22 of fp16), else rounded to the tiles' type, as
-// the output is.  Sums, maxima and states are fp32.
+// the tiles' is carried as hi + lo (2^-17 of bf16 pieces, 2^-22 of fp16); the
+// probabilities as two fp16 or three bf16 pieces where the output is fp32 (2^-22,
+// 2^-25: two bf16 pieces left an error of 2.1e-6 where fp32 sums have 4e-7), else
+// rounded to the tiles' type, as the output is.  Sums, maxima and states are fp32.
 //
 // Masked keys.  A key behind a row's position never meets its weight: the scores
 // are selected to -inf, V rows past the unit are zeroed, and a non-finite V element
@@ -418,6 +419,18 @@ __device__ __forceinline__ void restore_odd(const SharedParams& p, const ShPiece
   }
 }
 
+// Two weights as pieces of the tiles' type, each what the ones before left.
+template <bool kBf, int N>
+__device__ inline void pieces(float a, float b, uint32_t (&w)[N][4], int j) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    w[n][j] = pack2<kBf>(a, b);
+    const float2_t r = unpack2<kBf>(w[n][j]);
+    a -= r[0];
+    b -= r[1];
+  }
+}
+
 // The softmax step over N raw scores of a lane's row (kOther: the lanes that hold its
 // other keys): raises the running maximum m (log2 units) where it is passed by more
 // than 2^8 and says by what the sums shrink.
@@ -443,7 +456,7 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   using Tl = ShTile<KV, kBf>;
   constexpr int KB = Sh::KB, MT = Sh::MT, KS = Sh::KS, DT = Sh::DT, NCH = Sh::NCH, TPD = Sh::TPD, RPW = Sh::RPW,
                 NP = Sh::NP;
-  constexpr int EB = KV::kBytes;
+  constexpr int EB = KV::kBytes, kPieces = !kSplitP ? 1 : kBf ? 3 : 2;
   uint16_t* sK = reinterpret_cast<uint16_t*>(lds);
   uint16_t* sV = sK + 2 * Sh::TILE;
   const int lane = threadIdx.x & 63;
@@ -682,27 +695,23 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
     const float negm = m == -__builtin_inff() ? 0.0f : -m;
 #pragma unroll
     for (int ts = 0; ts < TS; ++ts) {
-      uint32_t w[4], wl[4];
+      uint32_t w[kPieces][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = 8 * (ts & 1) + 2 * j;
         const float p0 = fast_exp2(fmaf(st[ts >> 1][i], qscale, negm));
         const float p1 = fast_exp2(fmaf(st[ts >> 1][i + 1], qscale, negm));
         l += p0 + p1;
-        w[j] = pack2<kBf>(p0, p1);
-        if constexpr (kSplitP) {
-          const float2_t r = unpack2<kBf>(w[j]);
-          wl[j] = pack2<kBf>(p0 - r[0], p1 - r[1]);
-        }
+        pieces<kBf>(p0, p1, w, j);
       }
-      const u32x4_t pb = u32x4_t{w[0], w[1], w[2], w[3]};
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const uint64_t x0 = __builtin_bit_cast(uint64_t, vf[ts & 1][dt][0]),
                        x1 = __builtin_bit_cast(uint64_t, vf[ts & 1][dt][1]);
         const u32x4_t av = u32x4_t{(uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32)};
-        o[dt] = mfma32<kBf>(av, pb, o[dt]);
-        if constexpr (kSplitP) o[dt] = mfma32<kBf>(av, u32x4_t{wl[0], wl[1], wl[2], wl[3]}, o[dt]);
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n)
+          o[dt] = mfma32<kBf>(av, u32x4_t{w[n][0], w[n][1], w[n][2], w[n][3]}, o[dt]);
       }
       if (ts + 2 < TS) load_vf(ts + 2);
       __builtin_amdgcn_sched_barrier(0);
@@ -760,7 +769,7 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
   using Sh = ShShape<D>;
   using Tl = ShTile<KV, kBf>;
   constexpr int KT = kSharedThinTile, KS = D / 32, NDT = D / 16, NCH = Sh::NCH, TPD = Sh::TPD, NDMA = Sh::NDMA;
-  constexpr int EB = KV::kBytes;
+  constexpr int EB = KV::kBytes, kPieces = !kSplitP ? 1 : kBf ? 3 : 2;
   const int lane = threadIdx.x & 63;
   const int col = lane & 15, kg = lane >> 4;
   const char* kbase = static_cast<const char*>(p.k) + (int64_t)u.kvh * p.k_sh * EB;
@@ -884,7 +893,7 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
       }
     }
     const float negm = m == -__builtin_inff() ? 0.0f : -m;
-    uint32_t w[4], wl[4];
+    uint32_t w[kPieces][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -892,14 +901,9 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
         const float p0 = fast_exp2(fmaf(st[mt][2 * j], qscale, negm));
         const float p1 = fast_exp2(fmaf(st[mt][2 * j + 1], qscale, negm));
         l += p0 + p1;
-        w[mt * 2 + j] = pack2<kBf>(p0, p1);
-        if constexpr (kSplitP) {
-          const float2_t r = unpack2<kBf>(w[mt * 2 + j]);
-          wl[mt * 2 + j] = pack2<kBf>(p0 - r[0], p1 - r[1]);
-        }
+        pieces<kBf>(p0, p1, w, mt * 2 + j);
       }
     }
-    const u32x4_t pb = u32x4_t{w[0], w[1], w[2], w[3]};
     const int r0 = kg * 4 + (col >> 2);
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
@@ -910,8 +914,8 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
           (lds_short4m_t*)(sV + (r0 + 16) * D + (dm_vpos<D>(r0 + 16, c >> 3) << 3) + (c & 7)));
       const uint64_t x0 = __builtin_bit_cast(uint64_t, a0), x1 = __builtin_bit_cast(uint64_t, a1);
       const u32x4_t a = u32x4_t{(uint32_t)x0, (uint32_t)(x0 >> 32), (uint32_t)x1, (uint32_t)(x1 >> 32)};
-      o[dt] = mfma16<kBf>(a, pb, o[dt]);
-      if constexpr (kSplitP) o[dt] = mfma16<kBf>(a, u32x4_t{wl[0], wl[1], wl[2], wl[3]}, o[dt]);
+#pragma unroll
+      for (int n = 0; n < kPieces; ++n) o[dt] = mfma16<kBf>(a, u32x4_t{w[n][0], w[n][1], w[n][2], w[n][3]}, o[dt]);
     }
   }
 

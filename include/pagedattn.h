@@ -350,8 +350,8 @@ int pa_write_kv_scaled(pa_tensor_t* k_cache, pa_tensor_t* v_cache, const pa_tens
  * fp16, bf16 or FP8 E4M3 caches (k_scale, v_scale as the scaled entry points), q and
  * out fp32, fp16 or bf16, q 16-byte aligned, B <= 1024, NG <= 512, MB * BS < 2^31 - 1024,
  * D in {32, 64, 128, 256}.
- * Probabilities are carried in 16 bits where out is a 16-bit type, as 16-bit hi + lo
- * pairs where it is fp32 (an infinite V element may then give NaN in its place).
+ * Probabilities are carried in 16 bits where out is a 16-bit type, in two (fp16) or
+ * three (bf16) 16-bit pieces where it is fp32 (an infinite V element may then give NaN in its place).
  * workspace: device memory of paged_attention_shared_prefix_workspace_size(...)
  * bytes on the current device, 256-byte aligned, of this call alone.  No reference
  * counterpart (its decode reads each sequence's whole context,

@@ -91,7 +91,7 @@ def exact(c, scale):
     return out, A, es, count
 
 
-def check(pa, dev, c, out="f32", scale=None, k_scale=None, **kw):
+def check(pa, dev, c, out="f32", scale=None, wr=None, **kw):
     D = c["q"].shape[-1]
     scale = D**-0.5 if scale is None else scale
     t = {n: c[n].to(dev) for n in ("q", "k", "v", "bt", "ctx", "starts", "prefix")}
@@ -104,7 +104,7 @@ def check(pa, dev, c, out="f32", scale=None, k_scale=None, **kw):
     got = got.double().cpu().reshape(want.shape)
     split = 0.0 if c["qt"] == c["tile"] else (2.0**-22 if c["tile"] == "f16" else 2.0**-16)
     e = es * ((D + 8) * 2.0**-24 + split + 2.0**-23)
-    wr = HALF[c["tile"]] if out != "f32" else HALF[c["tile"]] ** 2
+    wr = wr if wr is not None else HALF[c["tile"]] if out != "f32" else HALF[c["tile"]] ** 2
     rel = 2 * e + (2 * n + 64) * 2.0**-24 + wr
     tol = A * rel[..., None]
     tol = tol + HALF[out] * (want.abs() + tol) + (2.0**-25 if out == "f16" else 0)
@@ -373,3 +373,9 @@ def test_long_table(pa, dev):
         print("tokens", n, flush=True)
         got = pa.paged_attention_shared_prefix(q, k, v, bt[:, :n // 16].clone(), i([n]), i([0, 1]), i([n // 2]), 0.1)
         assert (got - short).abs().max() <= tol * v.float().abs().max()
+
+
+@pytest.mark.parametrize("H,HKV,D,S,kv", [(8, 2, 128, 1, "bf16"), (8, 2, 64, 6, "bf16"), (8, 1, 256, 1, "bf16"), (8, 2, 128, 1, "fp8")])
+def test_single_precision(pa, dev, H, HKV, D, S, kv):
+    """fp32 results from bf16 pieces: the weights keep three of them, half a step of 2^-8 each, 2^-24 together."""
+    check(pa, dev, case(12, H, HKV, D, 16, kv=kv, q="bf16", S=S, seed=S + D, **RAGGED), "f32", wr=2.0**-24)
