@@ -239,7 +239,7 @@ struct RopeParams {
   int32_t q_blocks, kv_blocks;         // work-groups of the query heads, and of the keys' or the values'
   float k_scale, v_scale, k_rcp, v_rcp;
   float eps, inv_d;
-  FastDiv bs_div, q_slices, kv_slices;
+  FastDiv bs_div, q_heads, kv_heads;
 };
 
 // Pages of the cache moved, forked and compacted.  A cache is [L, NB, BS, row]

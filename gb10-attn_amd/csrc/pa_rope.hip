@@ -15,8 +15,14 @@
 // lane holds two chunks of eight elements chosen so that both elements of each
 // of its pairs are its own (chunks u and u + rot / 16; interleaved pairs are
 // neighbours): the rotation needs no exchange, the norm one sum over the D / 16
-// lanes of a row.  A lane group takes kRows heads of one token, all loaded
-// before the first is used, with the same eight cosines, sines and weights.
+// lanes of a row.  A lane group takes one head: two or four with the same cosines,
+// sines and weights were slower at nearly every size, since fewer waves are in
+// flight (32/8 heads of 128 in bf16, 1, 2 and 4 heads: 512 tokens 5.1, 5.6, 6.9 us;
+// 8192 tokens 43.7, 45.4, 47.0).
+//
+// HBM-bound where the tokens are many: 8192 tokens of 32/8 heads of 128, 251 MB read
+// and written, in 43.7 us (5.8 TB/s), into FP8 189 MB in 42; a launch and its chain of
+// dependent loads (position, table row) where they are few: 32 tokens 3.6 us.
 #include "pa_convert.hpp"
 
 #include <algorithm>
@@ -51,14 +57,14 @@ __device__ inline void divide8(float (&x)[8], float s, float r, bool exact, bool
 }
 
 // One work-group's share of the query, key or value heads: a group of LPR lanes (a
-// power of two, D / 16 of them in use) takes kRows heads of one token.  idx: the
-// thread among those of its kind.
-template <int ACT, int DST, int LPR, int kRows, int kKind>
-__device__ __forceinline__ void rope_heads(const RopeParams& p, uint32_t idx, const FastDiv& slices, int heads) {
+// power of two, D / 16 of them in use) takes one head of one token.  idx: the thread
+// among those of its kind.
+template <int ACT, int DST, int LPR, int kKind>
+__device__ __forceinline__ void rope_heads(const RopeParams& p, uint32_t idx, const FastDiv& heads) {
   const uint32_t grp = idx / LPR;
-  const uint32_t tl = fastdiv(grp, slices);  // token of this launch
+  const uint32_t tl = fastdiv(grp, heads);  // token of this launch
   if (tl >= (uint32_t)p.T) return;
-  const int head0 = (int)(grp - tl * slices.d) * kRows;
+  const int h = (int)(grp - tl * heads.d);
   const int64_t t = p.t_base + tl;
   const int u = (int)(idx % LPR);
   const bool on = u < p.D / 16;
@@ -75,23 +81,19 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, uint32_t idx, co
   const int64_t sh = kKind == kRopeQ ? p.q_sh : kKind == kRopeK ? p.key_sh : p.val_sh;
   const int64_t st = kKind == kRopeQ ? p.q_st : kKind == kRopeK ? p.key_st : p.val_st;
 
-  float x[kRows][16];
+  float x[16], c[8], d[8];
+  if (on) {
+    const int64_t off = t * st + (int64_t)h * sh;
+    load8<ACT>(src, off + a0, c);
+    load8<ACT>(src, off + a1, d);
+  } else {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    float c[8], d[8];
-    if (on && head0 + r < heads) {
-      const int64_t off = t * st + (int64_t)(head0 + r) * sh;
-      load8<ACT>(src, off + a0, c);
-      load8<ACT>(src, off + a1, d);
-    } else {
+    for (int e = 0; e < 8; ++e) c[e] = d[e] = 0.0f;
+  }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = d[e] = 0.0f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[r][e] = c[e];
-      x[r][8 + e] = d[e];
-    }
+  for (int e = 0; e < 8; ++e) {
+    x[e] = c[e];
+    x[8 + e] = d[e];
   }
   int64_t slot = 0;
   if constexpr (kKind != kRopeQ) slot = load_index(p.slots, p.slot_i64, t);
@@ -114,109 +116,104 @@ __device__ __forceinline__ void rope_heads(const RopeParams& p, uint32_t idx, co
     }
   }
 
+  if constexpr (kKind != kRopeV) {
+    if (w) {  // (the same for every lane)
+      float ss = 0.0f;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int h = head0 + r;
-    if constexpr (kKind != kRopeV) {
-      if (w) {  // (the same for every lane)
-        float ss = 0.0f;
+      for (int e = 0; e < 16; ++e) ss = fmaf(x[e], x[e], ss);
+      ss = group_sum<LPR>(ss);  // (every lane of the group takes part)
+      const float rms = 1.0f / __builtin_sqrtf(fmaf(ss, p.inv_d, p.eps));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) ss = fmaf(x[r][e], x[r][e], ss);
-        ss = group_sum<LPR>(ss);  // (every lane of the group takes part)
-        const float rms = 1.0f / __builtin_sqrtf(fmaf(ss, p.inv_d, p.eps));
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= rms * w0[e];
+        x[8 + e] *= rms * w1[e];
+      }
+    }
+  }
+  if (!on) return;
+  if constexpr (kKind != kRopeV) {
+    if (turned) {
+      if (p.interleaved) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[r][e] *= rms * w0[e];
-          x[r][8 + e] *= rms * w1[e];
+          const float a = x[2 * e], b = x[2 * e + 1];
+          x[2 * e] = a * cs[e] - b * sn[e];
+          x[2 * e + 1] = b * cs[e] + a * sn[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float a = x[e], b = x[8 + e];
+          x[e] = a * cs[e] - b * sn[e];
+          x[8 + e] = b * cs[e] + a * sn[e];
         }
       }
     }
-    if (!on || h >= heads) continue;
-    if constexpr (kKind != kRopeV) {
-      if (turned) {
-        if (p.interleaved) {
+  }
+  float lo[8], hi[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = x[r][2 * e], b = x[r][2 * e + 1];
-            x[r][2 * e] = a * cs[e] - b * sn[e];
-            x[r][2 * e + 1] = b * cs[e] + a * sn[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = x[r][e], b = x[r][8 + e];
-            x[r][e] = a * cs[e] - b * sn[e];
-            x[r][8 + e] = b * cs[e] + a * sn[e];
-          }
-        }
-      }
+  for (int e = 0; e < 8; ++e) {
+    lo[e] = x[e];
+    hi[e] = x[8 + e];
+  }
+  if constexpr (kKind == kRopeQ) {
+    const int64_t o = t * p.out_st + (int64_t)h * p.out_sh;
+    switch (p.out_dtype) {
+      case kF16: store8<kF16>(p.q_out, o + a0, lo); store8<kF16>(p.q_out, o + a1, hi); break;
+      case kBF16: store8<kBF16>(p.q_out, o + a0, lo); store8<kBF16>(p.q_out, o + a1, hi); break;
+      default: store8<kF32>(p.q_out, o + a0, lo); store8<kF32>(p.q_out, o + a1, hi); break;
     }
-    float lo[8], hi[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      lo[e] = x[r][e];
-      hi[e] = x[r][8 + e];
+  } else {
+    if (slot < 0 || slot >= p.nslots) return;
+    const uint32_t blk = fastdiv((uint32_t)slot, p.bs_div);
+    const uint32_t row = (uint32_t)slot - blk * (uint32_t)p.BS;
+    if (!p.unit_scale) {
+      const float s = kKind == kRopeV ? p.v_scale : p.k_scale, rc = kKind == kRopeV ? p.v_rcp : p.k_rcp;
+      const bool fast = kKind == kRopeV ? p.v_fast : p.k_fast, exact = kKind == kRopeV ? p.v_exact : p.k_exact;
+      divide8(lo, s, rc, exact, fast);
+      divide8(hi, s, rc, exact, fast);
     }
-    if constexpr (kKind == kRopeQ) {
-      const int64_t o = t * p.out_st + (int64_t)h * p.out_sh;
-      switch (p.out_dtype) {
-        case kF16: store8<kF16>(p.q_out, o + a0, lo); store8<kF16>(p.q_out, o + a1, hi); break;
-        case kBF16: store8<kBF16>(p.q_out, o + a0, lo); store8<kBF16>(p.q_out, o + a1, hi); break;
-        default: store8<kF32>(p.q_out, o + a0, lo); store8<kF32>(p.q_out, o + a1, hi); break;
-      }
-    } else {
-      if (slot < 0 || slot >= p.nslots) continue;
-      const uint32_t blk = fastdiv((uint32_t)slot, p.bs_div);
-      const uint32_t row = (uint32_t)slot - blk * (uint32_t)p.BS;
-      if (!p.unit_scale) {
-        const float s = kKind == kRopeV ? p.v_scale : p.k_scale, rc = kKind == kRopeV ? p.v_rcp : p.k_rcp;
-        const bool fast = kKind == kRopeV ? p.v_fast : p.k_fast, exact = kKind == kRopeV ? p.v_exact : p.k_exact;
-        divide8(lo, s, rc, exact, fast);
-        divide8(hi, s, rc, exact, fast);
-      }
-      void* c = kKind == kRopeV ? p.vc : p.kc;
-      const int64_t d = kKind == kRopeV ? (int64_t)blk * p.vc_sb + (int64_t)row * p.vc_st + (int64_t)h * p.vc_sh
-                                        : (int64_t)blk * p.kc_sb + (int64_t)row * p.kc_st + (int64_t)h * p.kc_sh;
-      store8<DST>(c, d + a0, lo);
-      store8<DST>(c, d + a1, hi);
-    }
+    void* c = kKind == kRopeV ? p.vc : p.kc;
+    const int64_t d = kKind == kRopeV ? (int64_t)blk * p.vc_sb + (int64_t)row * p.vc_st + (int64_t)h * p.vc_sh
+                                      : (int64_t)blk * p.kc_sb + (int64_t)row * p.kc_st + (int64_t)h * p.kc_sh;
+    store8<DST>(c, d + a0, lo);
+    store8<DST>(c, d + a1, hi);
   }
 }
 
 // Query heads' work-groups first, then keys', then values': a wave serves one kind
 // (with the kinds mixed in a wave it ran every kind's code: 8192 tokens of 32/8
 // heads of 128 into FP8 63 us, so 43).
-template <int ACT, int DST, int LPR, int kRows>
+template <int ACT, int DST, int LPR>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(const RopeParams p) {
   int b = blockIdx.x;
   if (b < p.q_blocks) {
-    rope_heads<ACT, DST, LPR, kRows, kRopeQ>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.q_slices, p.H);
+    rope_heads<ACT, DST, LPR, kRopeQ>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.q_heads);
   } else if ((b -= p.q_blocks) < p.kv_blocks) {
-    rope_heads<ACT, DST, LPR, kRows, kRopeK>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_slices, p.HKV);
+    rope_heads<ACT, DST, LPR, kRopeK>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_heads);
   } else {
     b -= p.kv_blocks;
-    rope_heads<ACT, DST, LPR, kRows, kRopeV>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_slices, p.HKV);
+    rope_heads<ACT, DST, LPR, kRopeV>(p, (uint32_t)b * kRopeThreads + threadIdx.x, p.kv_heads);
   }
 }
 
 // Lane groups per launch and kind: fewer than 2^27, so that thread indices stay below 2^31.
 constexpr int64_t kRopeMaxGroups = (int64_t)1 << 26;
 
-template <int ACT, int DST, int LPR, int kRows>
+template <int ACT, int DST, int LPR>
 static hipError_t launch_r(const RopeParams& p0, hipStream_t stream) {
   RopeParams p = p0;
-  const int64_t qs = (p.H + kRows - 1) / kRows, ks = (p.HKV + kRows - 1) / kRows;
-  p.q_slices = make_fastdiv((uint32_t)std::max<int64_t>(1, qs));
-  p.kv_slices = make_fastdiv((uint32_t)std::max<int64_t>(1, ks));
-  const int64_t step = std::max<int64_t>(1, kRopeMaxGroups / std::max<int64_t>(1, std::max(qs, ks)));
-  note_launch("pa::qk_norm_rope_kernel<%d, %d, %d, %d>", ACT, DST, LPR, kRows);
+  p.q_heads = make_fastdiv((uint32_t)std::max(1, p.H));
+  p.kv_heads = make_fastdiv((uint32_t)std::max(1, p.HKV));
+  const int64_t step = std::max<int64_t>(1, kRopeMaxGroups / std::max(1, std::max(p.H, p.HKV)));
+  note_launch("pa::qk_norm_rope_kernel<%d, %d, %d>", ACT, DST, LPR);
   for (int64_t t = 0; t < p0.T; t += step) {
     p.t_base = t;
     p.T = (int32_t)std::min<int64_t>(step, p0.T - t);
-    auto blocks = [&](int64_t slices) { return (int32_t)((p.T * slices * LPR + kRopeThreads - 1) / kRopeThreads); };
-    p.q_blocks = blocks(qs);
-    p.kv_blocks = blocks(ks);
-    hipLaunchKernelGGL((qk_norm_rope_kernel<ACT, DST, LPR, kRows>), dim3((unsigned)(p.q_blocks + 2 * p.kv_blocks)),
+    auto blocks = [&](int64_t heads) { return (int32_t)((p.T * heads * LPR + kRopeThreads - 1) / kRopeThreads); };
+    p.q_blocks = blocks(p.H);
+    p.kv_blocks = blocks(p.HKV);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<ACT, DST, LPR>), dim3((unsigned)(p.q_blocks + 2 * p.kv_blocks)),
                        dim3(kRopeThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -227,13 +224,10 @@ static hipError_t launch_r(const RopeParams& p0, hipStream_t stream) {
 template <int ACT, int DST>
 static hipError_t launch_r_d(const RopeParams& p, hipStream_t stream) {
   const int n = p.D / 16;
-  const bool many = (int64_t)p.T * (p.H + 2 * p.HKV) >= 16384;
-#define PA_ROPE(L) return many ? launch_r<ACT, DST, L, 4>(p, stream) : launch_r<ACT, DST, L, 1>(p, stream)
-  if (n <= 2) PA_ROPE(2);
-  if (n <= 4) PA_ROPE(4);
-  if (n <= 8) PA_ROPE(8);
-  PA_ROPE(16);
-#undef PA_ROPE
+  if (n <= 2) return launch_r<ACT, DST, 2>(p, stream);
+  if (n <= 4) return launch_r<ACT, DST, 4>(p, stream);
+  if (n <= 8) return launch_r<ACT, DST, 8>(p, stream);
+  return launch_r<ACT, DST, 16>(p, stream);
 }
 
 template <int ACT>

@@ -301,6 +301,7 @@ std::optional<at::Tensor> rows_of(const std::optional<at::Tensor>& t) {
 // `narrow`: what does not fit stays out of range), contiguous, on the device.
 at::Tensor index_of(const at::Tensor& t, const at::Device& dev, bool narrow) {
   const at::ScalarType ty = t.scalar_type();
+  if ((ty == at::kInt || (ty == at::kLong && !narrow)) && t.device() == dev && t.is_contiguous()) return t;
   if (narrow && ty == at::kLong) return t.to(dev).clamp(INT32_MIN, INT32_MAX).to(at::kInt).contiguous();
   const at::ScalarType want = narrow ? at::kInt : ty == at::kInt || ty == at::kLong ? ty : at::kLong;
   return t.to(dev, want).contiguous();
