@@ -105,52 +105,51 @@ __device__ inline int pages_of(const ForkParams& p, int32_t len) {
 
 // One wave's entry: the row's old pages are let go, the parent's whole pages are
 // counted once more and its pages kept aside, since another entry may replace the
-// parent's own row.  No table changes yet.
-__device__ inline void share_entry(const ForkParams& p, int i) {
+// parent's own row.  No table changes yet.  Returns the page that the parent has
+// begun, or -1.  (Both rows' lengths, then both rows' pages, come in one round trip
+// each: a fork of few rows is its chain of round trips.)
+__device__ inline int32_t share_entry(const ForkParams& p, int i) {
   const int lane = threadIdx.x & 63;
-  const int32_t row = p.rows[i];
   const int64_t NB = p.pool.num_blocks;
-  if (row < 0 || row >= p.R || !first_of_row(p.rows, i, row)) {
+  const int32_t row = p.rows[i], par = p.parents ? p.parents[i] : -1;
+  const bool first = first_of_row(p.rows, i, row);
+  if (row < 0 || row >= p.R || !first) {
     if (lane == 0) {
       p.ws_len[i] = -1;
       p.ws_last[i] = -1;
       p.result[i] = kForkInvalid;
     }
-    return;
+    return -1;
   }
+  const bool from = par >= 0 && par < p.R;
+  const int32_t old_len = p.lens[row], par_len = p.lens[from ? par : row];
   const int32_t* old = p.tables + row * p.tb_stride;
-  const int held = pages_of(p, p.lens[row]);
-  for (int j = lane; j < held; j += 64) {
-    const int32_t pg = old[j];
-    if (pg >= 0 && pg < NB) atomicAdd(p.refs + pg, -1);
+  const int32_t* src = p.tables + (from ? par : row) * p.tb_stride;
+  int32_t len = from ? max(par_len, 0) : 0, last = -1, res = par >= p.R ? kForkInvalid : kForkNone;
+  const int held = pages_of(p, old_len), n = pages_of(p, len);
+  bool bad = len > 0 && n == 0;
+  int32_t mine = -1;  // the parent's page number `lane`
+  for (int j = lane; j < max(held, n); j += 64) {
+    const int32_t pg = j < n ? src[j] : 0, was = j < held ? old[j] : -1;
+    if (j < n) p.ws_pages[(int64_t)i * p.MB + j] = pg;
+    if (was >= 0 && was < NB) atomicAdd(p.refs + was, -1);
+    bad |= j < n && (pg < 0 || pg >= NB);
+    mine = j < 64 ? pg : mine;
   }
-  const int32_t par = p.parents ? p.parents[i] : -1;
-  int32_t len = 0, last = -1, res = kForkNone;
-  if (par >= p.R) {
+  if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+    len = 0;
     res = kForkInvalid;
-  } else if (par >= 0) {
-    len = max(p.lens[par], 0);
-    const int n = pages_of(p, len);
-    const int32_t* src = p.tables + par * p.tb_stride;
-    bool bad = len > 0 && n == 0;
-    for (int j = lane; j < n; j += 64) bad |= src[j] < 0 || src[j] >= NB;
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
-      len = 0;
-      res = kForkInvalid;
-    } else {
-      const int whole = (int)fastdiv((uint32_t)len, p.bs_div);
-      for (int j = lane; j < n; j += 64) {
-        p.ws_pages[(int64_t)i * p.MB + j] = src[j];
-        if (j < whole) atomicAdd(p.refs + src[j], 1);
-      }
-      if (whole < n) last = src[whole];
-    }
+  } else {
+    const int whole = (int)fastdiv((uint32_t)len, p.bs_div);
+    for (int j = lane; j < whole; j += 64) atomicAdd(p.refs + (j < 64 ? mine : src[j]), 1);
+    if (whole < n) last = whole < 64 ? __shfl(mine, whole, 64) : src[whole];
   }
   if (lane == 0) {
     p.ws_len[i] = len;
     p.ws_last[i] = last;
     p.result[i] = res;
   }
+  return last;
 }
 
 __global__ __launch_bounds__(kPgThreads) void fork_share_kernel(const ForkParams p) {
@@ -181,20 +180,78 @@ __device__ inline int scan_block(int v, int& total, int* s_part) {
   return before + x - v;
 }
 
-// One work-group (kShare: with share_entry() of every entry first, which saves a launch
-// where there are few table entries to walk).  A begun page that nobody holds any more goes to the lowest
-// entry forked from it; every other entry with a begun page gets a copy, in the
-// lowest free page, in the order of the entries.  Free pages are found in one
-// pass over the counts that ends when there are enough.
+// The first pages that nobody holds, as many as `need`: put(rank, page) in ascending
+// order, in one pass over the counts that ends when there are enough.  Returns how
+// many there were.
+template <typename Put>
+__device__ inline int find_free(const ForkParams& p, int need, int* s_part, const Put& put) {
+  const int64_t NB = p.pool.num_blocks;
+  int found = 0;
+  for (int64_t b0 = 0; b0 < NB && found < need; b0 += 4 * kScan) {
+    int32_t r[4];
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t pg = b0 + 4 * (int)threadIdx.x + k;
+      r[k] = pg < NB ? load_now(p.refs + pg) : 1;
+      n += r[k] == 0;
+    }
+    int total;
+    int rank = found + scan_block(n, total, s_part);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (r[k] != 0) continue;
+      if (rank < need) put(rank, (int32_t)(b0 + 4 * (int)threadIdx.x + k));
+      ++rank;
+    }
+    found += total;
+  }
+  return min(found, need);
+}
+
+// Pages for the entries, in one work-group.  A begun page that nobody holds any more
+// goes to the lowest entry forked from it; every other entry with a begun page gets
+// a copy, in the lowest free page, in the order of the entries.
+//
+// Up to kScan entries, one a thread, compared through LDS (kShare: share_entry() of
+// each before, which saves a launch where every wave has one at most).
 template <bool kShare>
-__global__ __launch_bounds__(kScan) void fork_alloc_kernel(const ForkParams p) {
+__global__ __launch_bounds__(kScan) void fork_few_kernel(const ForkParams p) {
+  __shared__ int s_part[kScan / 64];
+  __shared__ int32_t s_last[kScan], s_free[kScan];
+  const int i = threadIdx.x;
+  if constexpr (kShare) {
+    for (int k = i >> 6; k < p.N; k += kScan / 64) {
+      const int32_t last = share_entry(p, k);
+      if ((i & 63) == 0) s_last[k] = last;
+    }
+  } else {
+    if (i < p.N) s_last[i] = p.ws_last[i];
+  }
+  __syncthreads();
+  const int32_t last = i < p.N ? s_last[i] : -1;
+  bool takes = last >= 0 && load_now(p.refs + last) == 0;
+  if (takes) {
+    for (int k = 0; k < i; ++k) takes = takes && s_last[k] != last;
+  }
+  const bool wants = last >= 0 && !takes;
+  __syncthreads();  // the counts of begun pages have been read
+  if (takes) atomicExch(p.refs + last, 1);
+  int need;
+  const int rank = scan_block(wants ? 1 : 0, need, s_part);
+  const int found = find_free(p, need, s_part, [&](int at, int32_t pg) { s_free[at] = pg; });
+  __syncthreads();
+  if (i >= p.N) return;
+  const int32_t fresh = wants && rank < found ? s_free[rank] : -1;
+  p.ws_new[i] = fresh;
+  if (fresh >= 0) atomicExch(p.refs + fresh, 1);
+  if (wants) p.result[i] = fresh >= 0 ? fresh : kForkNoPage;
+}
+
+// The same for any number of entries, compared through ws_owner.
+__global__ __launch_bounds__(kScan) void fork_many_kernel(const ForkParams p) {
   __shared__ int s_part[kScan / 64];
   const int tid = threadIdx.x;
-  const int64_t NB = p.pool.num_blocks;
-  if constexpr (kShare) {
-    for (int i = tid >> 6; i < p.N; i += kScan / 64) share_entry(p, i);
-    __syncthreads();
-  }
   for (int i = tid; i < p.N; i += kScan) {
     const int32_t last = p.ws_last[i];
     if (last >= 0) atomicExch(p.ws_owner + last, INT32_MAX);
@@ -224,26 +281,8 @@ __global__ __launch_bounds__(kScan) void fork_alloc_kernel(const ForkParams p) {
   }
   __syncthreads();
   // ws_owner's use is over: its first entries take the free pages.
-  int found = 0;
-  for (int64_t b0 = 0; b0 < NB && found < need; b0 += 4 * kScan) {
-    int32_t r[4];
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t pg = b0 + 4 * tid + k;
-      r[k] = pg < NB ? load_now(p.refs + pg) : 1;
-      n += r[k] == 0;
-    }
-    int total;
-    int rank = found + scan_block(n, total, s_part);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (r[k] != 0) continue;
-      if (rank < need) atomicExch(p.ws_owner + rank, (int32_t)(b0 + 4 * tid + k));
-      ++rank;
-    }
-    found += total;
-  }
+  const int found =
+      find_free(p, need, s_part, [&](int at, int32_t pg) { atomicExch(p.ws_owner + at, pg); });
   __syncthreads();
   for (int i = tid; i < p.N; i += kScan) {
     const int rank = p.ws_new[i];
@@ -315,21 +354,27 @@ hipError_t launch_free(const ForkParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Most table entries that one work-group walks for a fork: 8 entries of tables of 16
-// pages 13.1 us in three launches, 11.0 in two; 64 of 128 22.8, and 37.8 in two.
-constexpr int64_t kForkFused = 1024;
+// Most entries that the allocating work-group shares itself, a wave each (in two
+// launches and in three, tables of 16 pages: 8 entries 8.6 and 10.3 us, 16 entries 8.9
+// and 10.3; 32 entries 11.2 both, 64 entries 15.0 and 12.3).
+constexpr int kForkFused = kScan / 64;
 
 hipError_t launch_fork(const ForkParams& p, hipStream_t stream) {
   hipError_t e;
-  if ((int64_t)p.N * p.MB <= kForkFused) {
-    note_launch("pa::fork_alloc_kernel<true>");
-    hipLaunchKernelGGL(fork_alloc_kernel<true>, dim3(1), dim3(kScan), 0, stream, p);
+  if (p.N <= kForkFused) {
+    note_launch("pa::fork_few_kernel<true>");
+    hipLaunchKernelGGL(fork_few_kernel<true>, dim3(1), dim3(kScan), 0, stream, p);
   } else {
     note_launch("pa::fork_share_kernel");
     hipLaunchKernelGGL(fork_share_kernel, dim3((unsigned)((p.N + 3) / 4)), dim3(kPgThreads), 0, stream, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    note_launch("pa::fork_alloc_kernel<false>");
-    hipLaunchKernelGGL(fork_alloc_kernel<false>, dim3(1), dim3(kScan), 0, stream, p);
+    if (p.N <= kScan) {
+      note_launch("pa::fork_few_kernel<false>");
+      hipLaunchKernelGGL(fork_few_kernel<false>, dim3(1), dim3(kScan), 0, stream, p);
+    } else {
+      note_launch("pa::fork_many_kernel");
+      hipLaunchKernelGGL(fork_many_kernel, dim3(1), dim3(kScan), 0, stream, p);
+    }
   }
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int64_t copies = std::min<int64_t>((int64_t)p.N * p.pool.planes * page_items(p.pool), kMaxGrid);

@@ -394,3 +394,25 @@ def test_numbers_past_32_bits(pa, dev, monkeypatch, tmp_path):
         assert got.tolist() == [-3, -3, -1] and ctx.tolist() == [8, 0, 0] and refs.tolist() == [1, 1] + [0] * 6
         pa.free_sequences(bt, ctx, refs, torch.tensor([2**32, -2**33]), 4)
         assert ctx.tolist() == [8, 0, 0] and refs.tolist() == [1, 1] + [0] * 6
+
+
+@pytest.mark.parametrize("R,MB,most", [(9, 100, 9), (40, 150, 40), (700, 3, 700)])
+def test_fork_long_and_many_rows(pa, dev, R, MB, most):
+    """Tables longer than a wave, and batches that take one launch more: steps in place, with rows emptied,
+    shared and begun pages, and at the end more copies than pages."""
+    rng = np.random.default_rng(MB)
+    BS = 2
+    lens = [int(x) for x in rng.integers(0, MB * BS + 1, R)]
+    NB = sum(-(-n // BS) for n in lens) + R // 3
+    bt, ctx, refs = state(R, MB, NB, BS, lens, rng)
+    for _ in range(3):
+        N = int(rng.integers(most // 2, most + 1))
+        rows = [int(x) for x in rng.permutation(R)[:N]]
+        parents = [int(x) for x in rng.integers(-1, R, N)]
+        run_fork(pa, dev, "f16", (1, NB, BS, 1, 32), bt, ctx, refs, parents, rows)
+        assert (refs >= 0).all()
+    free = int((refs == 0).sum())
+    odd = [r for r in range(R) if ctx[r] % BS]
+    if odd:
+        spare = [r for r in range(R) if r != odd[0]][:free + 5]
+        run_fork(pa, dev, "f16", (1, NB, BS, 1, 32), bt, ctx, refs, [odd[0]] * len(spare), spare)
