@@ -176,14 +176,28 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, ShTables& s, int32_t* 
     group(g, p.group_starts[g], g < p.NG ? p.group_starts[g + 1] : 0, g < p.NG ? p.prefix_lens[g] : 0);
   fault = __syncthreads_or(bad);
   if (fault) return {0, 0, 4};
+  // Costs of the groups, then of the sequences, and their prefix sums.
   int carry = 0;
-  auto scan = [&](int i, int n, int c, int32_t* cum) {
+  const int n = p.NG + p.B;
+  for (int i0 = 0; i0 < n; i0 += kShThreads) {
+    const int i = i0 + tid, b = i - p.NG;
+    int c = 0;
+    if (i < p.NG) {
+      if (s_len[i] > 0 && s_len[i] <= maxctx)
+        c = p.HKV * row_blocks((s.start[i + 1] - s.start[i]) * p.SG) * wide_cost(wide_tiles(s_len[i]));
+    } else if (i < n) {
+      const int g = group_of(s.start, p.NG, b);
+      const int P = g < 0 ? 0 : s_len[g], ctx = s.ctx[b];
+      s.pre[b] = P;
+      if (ctx > P && ctx <= maxctx) c = p.HKV * p.own_rb * own_cost(p, own_tiles(p, ctx - own_first(P)));
+    }
     int x = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int y = __shfl_up(x, o, 64);
       if (lane >= o) x += y;
     }
+    if (i0 > 0) __syncthreads();  // s_tmp has been read
     if (lane == 63) s_tmp[wave] = x;
     __syncthreads();
     int before = carry;
@@ -192,30 +206,11 @@ __device__ inline ShPlan plan_scan(const SharedParams& p, ShTables& s, int32_t* 
       before += w < wave ? s_tmp[w] : 0;
       carry += s_tmp[w];
     }
-    if (i < n) cum[i] = before + x - c;
-    __syncthreads();
-  };
-  for (int i0 = 0; i0 < p.NG; i0 += kShThreads) {
-    const int g = i0 + tid;
-    int c = 0;
-    if (g < p.NG && s_len[g] > 0 && s_len[g] <= maxctx)
-      c = p.HKV * row_blocks((s.start[g + 1] - s.start[g]) * p.SG) * wide_cost(wide_tiles(s_len[g]));
-    scan(g, p.NG, c, s.cum);
+    if (i < n) s.cum[i] = before + x - c;
   }
-  const int own = carry;
-  for (int i0 = 0; i0 < p.B; i0 += kShThreads) {
-    const int b = i0 + tid;
-    int c = 0;
-    if (b < p.B) {
-      const int g = group_of(s.start, p.NG, b);
-      const int P = g < 0 ? 0 : s_len[g], ctx = s.ctx[b];
-      s.pre[b] = P;
-      if (ctx > P && ctx <= maxctx) c = p.HKV * p.own_rb * own_cost(p, own_tiles(p, ctx - own_first(P)));
-    }
-    scan(b, p.B, c, s.cum + p.NG);
-  }
-  if (tid == 0) s.cum[p.NG + p.B] = carry;
+  if (tid == 0) s.cum[n] = carry;
   __syncthreads();
+  const int own = s.cum[p.NG];
   const int even = (carry + p.wgs - 1) / p.wgs;
   return {carry, own, max(kSharedMinShare, (even + 3) & ~3)};
 }
