@@ -28,6 +28,24 @@
 // Both compute S^T = K Q^T, whose accumulator layout is the operand layout of
 // O^T += V^T P^T: the probabilities stay in registers.
 //
+// What bounds it.  A CU takes a wide tile of 128 rows and 64 keys of 128 per 1.3 us
+// (0.83 PFLOP/s over the card, where a large library product reaches 1.2):
+// neither the matrix cores (28 % busy), the vector ALU (35 %) nor LDS (23 %) is full,
+// but a wave's chain (scores, maximum, weights, products) and the two waves of a SIMD
+// fill each other's gaps only in part; one work-group a CU takes 1.9 us a tile.  Eight
+// waves sharing a tile (256 rows, one work-group a CU) ran at the same rate a row with
+// a state of twice the size to write, and alternating their phases did not fit the
+// registers.  Thin tiles run at the memory's rate (64 x 4096 tokens of 32/8 heads of
+// 128 in bf16: 183 us, 5.9 TB/s).  A call is 2.4 us until its line is known, 2 to 6
+// until a first tile (FP8 codes and long tables the most), and the merge, 4 us or the
+// time of the states' bytes (8192 rows over 512 pieces of 128: 42 MB, 12 us).
+//
+// Variants, with both sides measured.  Thin units up to 16 rows: 64 x 4096 tokens,
+// 32/8 heads of 128, 4 rows 183 us (wide 200), 16 rows 198 (210); at 32 rows a thin
+// unit of two row blocks gained 2 to 8 % at D <= 128 and lost 45 % at 256.  Pages of a
+// multiple of 16 tokens: one page id a wave (128 rows over 8192 tokens 48.0 us; a page
+// id a row, taken for other sizes, 49.1).
+//
 // Types.  FP8 codes widen exactly to the 16-bit type of q.  q of another type than
 // the tiles' is carried as hi + lo (2^-17 of bf16 pieces, 2^-22 of fp16); the
 // probabilities as two fp16 or three bf16 pieces where the output is fp32 (2^-22,
@@ -634,6 +652,8 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
       for (int i = 0; i < 16; ++i) st[mt][i] = 0.0f;
     }
     __builtin_amdgcn_sched_barrier(0);
+    // (A wave at its scores goes before the CU's other work-group at its softmax.)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -644,6 +664,7 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
       if (ks + WK < KS) load_a(ks + WK);
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     load_vf(0);
     if constexpr (TS > 1) load_vf(1);
     __builtin_amdgcn_sched_barrier(0);
