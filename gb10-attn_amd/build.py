@@ -120,8 +120,7 @@ def resources() -> str:
     cols = list(_REMARK_KEYS.values())
     out = ["| kernel | file | " + " | ".join(cols) + " |", "|---|---|" + "---|" * len(cols)]
     for r, n in zip(rows, names):
-        n = n.replace("(pa::DecodeParams)", "").replace("(pa::PrefillParams)", "").replace(
-            "(pa::ReduceParams)", "").replace("(pa::WriteParams)", "")
+        n = re.sub(r"\(pa::\w+Params\)", "", n)
         out.append(f"| `{n}` | {r['file']} | " + " | ".join(r.get(c, "") for c in cols) + " |")
     return "\n".join(out) + "\n"
 

@@ -339,10 +339,11 @@ constexpr int kSharedWideTile = 64;   // keys of a tile of either
 constexpr int kSharedThinTile = 32;
 // Cost of a tile and of a unit's start (its first loads, and its state's store), in
 // parts of 0.3 us of a work-group; a thin tile is a wave's, four at a time.  (A wide
-// tile takes 1.8 to 2.6 us with two work-groups on a CU, a start 5 to 8: taken for 10
-// parts instead of 20, the work-groups with many short units ended last and a call of
-// 32 x 4 rows of 64/8 heads over 16384 tokens took 129 us, not 113.)
-constexpr int kSharedWideCost = 7, kSharedWideStart = 20;
+// tile takes 1.8 to 2.6 us with two work-groups on a CU, a start 5 to 8.  At 10 parts a
+// start the work-groups with many short units ended last, 32 x 4 rows of 64/8 heads
+// over 16384 tokens in 113.6 us; 107.5 at 14 to 17; at 20 64 rows of 12 heads over 2048
+// tokens took 17.8 us, not 16.7.)
+constexpr int kSharedWideCost = 7, kSharedWideStart = 16;
 constexpr int kSharedThinCost = 3, kSharedThinStart = 2;
 constexpr int kSharedMinShare = 4 * kSharedThinCost;  // a wave's share holds the start of a tile
 constexpr int kSharedMeta = 8;  // prefix, context, the group's first sequence, its rows, cost before its units

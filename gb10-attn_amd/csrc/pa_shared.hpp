@@ -30,7 +30,7 @@
 //
 // What bounds it.  A CU takes a wide tile of 128 rows and 64 keys of 128 per 1.3 us
 // (0.83 PFLOP/s over the card, where a large library product reaches 1.2):
-// neither the matrix cores (28 % busy), the vector ALU (35 %) nor LDS (23 %) is full,
+// neither the matrix cores (27 % busy), the vector ALU (32 %) nor LDS (22 %) is full,
 // but a wave's chain (scores, maximum, weights, products) and the two waves of a SIMD
 // fill each other's gaps only in part; one work-group a CU takes 1.9 us a tile.  Eight
 // waves sharing a tile (256 rows, one work-group a CU) ran at the same rate a row with
@@ -472,7 +472,11 @@ __device__ __forceinline__ void wide_piece(const SharedParams& p, const ShPiece&
   constexpr int EB = KV::kBytes, kPieces = !kSplitP ? 1 : kBf ? 3 : 2;
   uint16_t* sK = reinterpret_cast<uint16_t*>(lds);
   uint16_t* sV = sK + 2 * Sh::TILE;
-  const int lane = threadIdx.x & 63;
+  int lane = threadIdx.x & 63;
+  // What follows from the lane is made anew each piece where registers are short, instead
+  // of kept in scratch meanwhile (64/8 heads of 128 in FP8 111.3 -> 109.6 us; 12 heads of
+  // 64, which have registers to spare, 17.8 -> 18.8).
+  if constexpr (D >= 128) asm volatile("" : "+v"(lane));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hh = lane >> 5;
 
@@ -786,7 +790,8 @@ __device__ __forceinline__ void thin_piece(const SharedParams& p, const ShPiece&
   using Tl = ShTile<KV, kBf>;
   constexpr int KT = kSharedThinTile, KS = D / 32, NDT = D / 16, NCH = Sh::NCH, TPD = Sh::TPD, NDMA = Sh::NDMA;
   constexpr int EB = KV::kBytes, kPieces = !kSplitP ? 1 : kBf ? 3 : 2;
-  const int lane = threadIdx.x & 63;
+  int lane = threadIdx.x & 63;
+  if constexpr (D >= 128) asm volatile("" : "+v"(lane));  // (as wide_piece)
   const int col = lane & 15, kg = lane >> 4;
   const char* kbase = static_cast<const char*>(p.k) + (int64_t)u.kvh * p.k_sh * EB;
   const char* vbase = static_cast<const char*>(p.v) + (int64_t)u.kvh * p.v_sh * EB;

@@ -240,3 +240,22 @@ def test_python_paths_agree(pa, dev, monkeypatch, tmp_path):
     for x, y in zip(calls(), want):
         assert x.dtype == y.dtype and torch.equal(x, y)
     refusals()
+
+
+def test_more_heads_than_one_launch(pa, dev):
+    """2^21 tokens of 40 heads, taken in two launches: as calls of their parts."""
+    T, H, HKV, D, BS = (1 << 21) + 7, 40, 1, 16, 16
+    qkv = torch.randn((T, H + 2 * HKV, D), device=dev, dtype=torch.bfloat16)
+    q, k, v = qkv[:, :H], qkv[:, H:H + HKV], qkv[:, H + HKV:]
+    w = (torch.randn(D, device=dev) * 0.2 + 1).bfloat16()
+    cs = table(500, D, torch.float32).to(dev)
+    pos, slots = torch.arange(T, device=dev) % 500, torch.arange(T, device=dev).flip(0)
+    new = lambda: [torch.zeros((T // BS + 1, BS, HKV, D), dtype=torch.bfloat16, device=dev) for _ in range(2)]  # noqa: E731
+    a, b = new(), new()
+    print("two launches", T, flush=True)
+    got = pa.qk_norm_rope_write_kv(q, k, v, *a, slots, cs, pos, q_weight=w, k_weight=w)
+    for i in range(0, T, 1 << 19):
+        s = slice(i, i + (1 << 19))
+        part = pa.qk_norm_rope_write_kv(q[s], k[s], v[s], *b, slots[s], cs, pos[s], q_weight=w, k_weight=w)
+        assert torch.equal(got[s], part)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[1].flatten(0, 1)[:T].any(-1).any(-1).all()
